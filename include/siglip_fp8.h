@@ -85,7 +85,9 @@ enum {
     SL8_FLAG_NO_ACTIVATION = 4,
     /* FC1: GELU through the hardware tanh (tanh.approx.f32, relative error ~2^-11): one special-function operation
      * per element instead of two.  |error| <= ~2.5e-4 |x| against the exact form; off by default. */
-    SL8_FLAG_GELU_HW_TANH = 8
+    SL8_FLAG_GELU_HW_TANH = 8,
+    /* sl8_linear_scaled: GELU(tanh) on the result, as FC1 has it by default. */
+    SL8_FLAG_GELU = 16
 };
 
 /* Which kernel variant the dispatch table picks for a problem. */
@@ -225,6 +227,42 @@ int sl8_quantize_e4m3(sl8_handle_t h, const void* x, int dtype, int64_t rows, in
 int sl8_layernorm_quantize_e4m3(sl8_handle_t h, const void* x, int dtype, int64_t rows, int cols, int64_t ld,
                                 const float* gamma, const float* beta, float eps, const float* scale,
                                 void* out, int64_t ld_out, sl8_stream_t stream);
+
+/* ---- 8-bit operands with a scale for each row --------------------------------------------
+ * No counterpart in the reference, whose operands are raw e4m3 codes.  A row of A is a token, a row of B an output channel:
+ * the codes of a row are multiples of a scale of its own, row_scales[r] (fp32, contiguous), so one large token or channel
+ * costs the others nothing.  Codes are int8 or e4m3, the same on both sides of a product. */
+enum { SL8_CODE_E4M3 = 0, SL8_CODE_INT8 = 1 };
+
+/* row_scales[r] = max |x[r, :]| / 127 (int8) or / 448 (e4m3), 1 for a row of zeros, never below 2^-126;
+ * out[r, c] = round(x[r, c] * (1 / row_scales[r])), ties to even: an activation, or weights [N, K].  A row with an infinity or a
+ * NaN gets the scale NaN (and no meaningful codes), so that whatever is computed from it is NaN, and no other row is touched.
+ * x fp32 or bf16, any number of columns; fastest where cols is a multiple of 8 and the rows of x start on 16-byte, those of out on
+ * 8-byte boundaries. */
+int sl8_quantize_rows(sl8_handle_t h, const void* x, int dtype, int64_t rows, int cols, int64_t ld, int code_type,
+                      void* out, int64_t ld_out, float* row_scales, sl8_stream_t stream);
+
+/* RMS norm with the residual's addition in front of it and the quantisation behind it:
+ *     h = x + residual (h = x where residual is NULL), y = h * gamma * rsqrt(mean(h^2) + eps)
+ * x, residual and sum are of type `dtype`, each with a leading dimension of its own; h is not rounded before it is used, statistics
+ * are fp32.  With a residual, sum receives h (rounded once to `dtype`): the new residual stream.  sum may be x or the residual itself
+ * (same address and leading dimension), but not overlap them otherwise.  gamma fp32 [cols] (NULL = 1).
+ *   row_scales given: codes and a scale for each row of y, as sl8_quantize_rows makes them (scale must be NULL);
+ *   row_scales NULL:  e4m3 codes e4m3_sat_rne(y * (1 / *scale)), one scale for all (NULL = 1): the operand of the layers above.
+ * A row whose sum of squares is beyond fp32, or which holds an infinity or a NaN, comes out as NaN: its scale, or its codes. */
+int sl8_rmsnorm_quantize(sl8_handle_t h, const void* x, int dtype, int64_t rows, int cols, int64_t ld,
+                         const void* residual, int64_t ld_res, void* sum, int64_t ld_sum,
+                         const float* gamma, float eps, int code_type, const float* scale,
+                         void* out, int64_t ld_out, float* row_scales, sl8_stream_t stream);
+
+/* D[m, n] = bf16( f( acc[m, n] * scale_a[m] * scale_b[n] + bias[n] ) ), acc = sum over k of A[m, k] * B[n, k]; f is the identity, or
+ * GELU(tanh) with SL8_FLAG_GELU.  A [M, K] and B [N, K] hold codes of `code_type`; int8 products are summed exactly in 32 bits (K at most
+ * 131 071), e4m3 products in fp32.  scale_a fp32 [M], scale_b fp32 [N], neither NULL; bias bf16 [N] (fp32 with SL8_FLAG_BIAS_F32) or
+ * NULL.  Alignment rules, variants and watchdog of the layers above.  Few rows (one token each of some sequences) take kernels of
+ * their own, which stream the weights; sl8_set_variant forces them off. */
+int sl8_linear_scaled(sl8_handle_t h, const void* A, int64_t lda, const void* B, int64_t ldb, int code_type,
+                      const float* scale_a, const float* scale_b, const void* bias,
+                      void* D, int64_t ldd, int64_t M, int N, int K, unsigned flags, sl8_stream_t stream);
 
 /* ---- the same three layers with HOST operands ------------------------------------------
  * What each reference main() does around its launch (upload operands, launch, download

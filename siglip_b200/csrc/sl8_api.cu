@@ -11,6 +11,7 @@
 
 #include "sl8_internal.h"
 #include "sl8_dispatch_table.h"
+#include "sl8_few.h"
 
 namespace {
 
@@ -55,7 +56,11 @@ inline bool aligned16(const void* p) { return sl8_aligned16(p); }
 
 // ---- dispatch -------------------------------------------------------------------------
 // The table is generated from a sweep on B200 (python -m siglip_b200.sweep); what it does not hold is answered by a cost model.
+// (beside the layers of the header, inside the library: operands with a scale per row)
+enum : int { kOpInt8 = sl8::OP_INT8, kOpE4M3 = sl8::OP_E4M3 };
 int kernel_slot(int op, int out_dtype) {
+    if (op == kOpInt8) return sl8::K_INT8;
+    if (op == kOpE4M3) return sl8::K_E4M3;
     if (op == SL8_OP_PATCH_EMBED) return sl8::K_PE;
     if (op == SL8_OP_FC2_RESIDUAL) return sl8::K_FC2;
     return out_dtype == SL8_OUT_E4M3 ? sl8::K_FC1_E4M3 : sl8::K_FC1_BF16;
@@ -109,6 +114,7 @@ int cheapest_variant(sl8_handle_t h, CostClass cls, int slot, long long M, int N
 
 int pick_variant(sl8_handle_t h, int op, int out_dtype, long long M, int N, int K, unsigned flags) {
     const int slot = kernel_slot(op, out_dtype);
+    if (sl8::op_scaled(op)) return cheapest_variant(h, (flags & SL8_FLAG_NO_ACTIVATION) ? COST_NONE : COST_GELU, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_NO_ACTIVATION)) return cheapest_variant(h, COST_NONE, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_GELU_HW_TANH)) return cheapest_variant(h, COST_TANH, slot, M, N, K);
     // A (layer, N, K) the committed sweep covers: the row with the largest m_min <= M decides.
@@ -131,7 +137,7 @@ struct Problem {
     int out_dtype;
     const void *A, *B;
     long long lda, ldb;
-    const float *scale_a, *scale_b, *out_scale;
+    const float *scale_a, *scale_b, *out_scale;    // scaled operands: fp32 [M] and [N]
     const void* bias;
     const void* side;
     long long ld_side;
@@ -157,7 +163,7 @@ int validate(sl8_handle_t h, const Problem& q) {
 #endif
     if (q.flags & ~(unsigned)(SL8_FLAG_BIAS_F32 | SL8_FLAG_PE_F32_ADD | SL8_FLAG_NO_ACTIVATION | SL8_FLAG_GELU_HW_TANH | kDiagBits))
         return fail(h, SL8_ERR_INVALID_VALUE, "unknown flag bits");
-    if ((q.flags & (SL8_FLAG_NO_ACTIVATION | SL8_FLAG_GELU_HW_TANH)) && q.op != SL8_OP_FC1_GELU)
+    if ((q.flags & (SL8_FLAG_NO_ACTIVATION | SL8_FLAG_GELU_HW_TANH)) && q.op != SL8_OP_FC1_GELU && !sl8::op_scaled(q.op))
         return fail(h, SL8_ERR_INVALID_VALUE, "SL8_FLAG_NO_ACTIVATION / SL8_FLAG_GELU_HW_TANH belong to the FC1 entry points");
     if ((q.flags & SL8_FLAG_NO_ACTIVATION) && (q.flags & SL8_FLAG_GELU_HW_TANH))
         return fail(h, SL8_ERR_INVALID_VALUE, "SL8_FLAG_NO_ACTIVATION and SL8_FLAG_GELU_HW_TANH exclude each other");
@@ -179,6 +185,11 @@ int validate(sl8_handle_t h, const Problem& q) {
         if (!q.side) return fail(h, SL8_ERR_INVALID_VALUE, "residual must not be NULL");
         if (q.ld_side < q.N) return fail(h, SL8_ERR_INVALID_VALUE, "ldr smaller than N");
         if (!aligned16(q.side) || (q.ld_side * 2) % 16) return fail(h, SL8_ERR_ALIGNMENT, "residual must be 16-byte aligned with a 16-byte pitch");
+    }
+    if (sl8::op_scaled(q.op)) {
+        if (!q.scale_a || !q.scale_b) return fail(h, SL8_ERR_INVALID_VALUE, "scale_a and scale_b must not be NULL");
+        // 128^2 * K < 2^31: no sum of int8 products leaves 32 bits
+        if (q.op == kOpInt8 && q.K > 131071) return fail(h, SL8_ERR_UNSUPPORTED, "int8 sums of more than 131071 products exceed 32 bits");
     }
     if (q.bias && !aligned16(q.bias)) return fail(h, SL8_ERR_ALIGNMENT, "bias must be 16-byte aligned");
     if (q.scale_a && (reinterpret_cast<uintptr_t>(q.scale_a) & 3u)) return fail(h, SL8_ERR_ALIGNMENT, "scale pointers must be 4-byte aligned");
@@ -247,12 +258,40 @@ int grid_for(sl8_handle_t h, const VariantEntry* v, int slot, int num_tiles) {
     return clusters * v->cg;
 }
 
+// Few rows of operands with a scale per row (sl8_few.cu).  The caller holds h->mu; the problem has been validated.
+int run_few(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
+    sl8::FewParams p = {};
+    p.M = static_cast<int>(q.M);
+    p.N = q.N;
+    p.k_blocks = (q.K + 127) / 128;
+    p.last_kblock_mmas = (q.K - (p.k_blocks - 1) * 128 + 31) / 32;
+    p.row_scales = q.scale_a;
+    p.col_scales = q.scale_b;
+    p.bias = q.bias;
+    p.D = q.D;
+    p.ldd = q.ldd;
+    p.flags = q.flags | (h->test_drop_b ? sl8::FLAG_TEST_DROP_B : 0u);
+    p.wait_budget_us = h->wait_budget_us;
+    p.status = h->d_status;
+    CUtensorMap map_a, map_b;
+    int rc = encode_2d(h, &map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.B, (unsigned long long)q.K, (unsigned long long)q.N,
+                       (unsigned long long)q.ldb, 128, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    if (rc != SL8_OK) return rc;
+    rc = encode_2d(h, &map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.A, (unsigned long long)q.K, (unsigned long long)q.M,
+                   (unsigned long long)q.lda, 128, (unsigned)sl8::few_tile_rows(p.M), CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+    if (rc != SL8_OK) return rc;
+    h->last_grid = 0;        // these kernels write no trace records
+    const cudaError_t e = sl8::few_launch(q.op == kOpInt8, sl8::few_split(h->sm_count, q.N, p.k_blocks), map_b, map_a, p, stream);
+    return e == cudaSuccess ? SL8_OK : fail_cuda(h, e, "kernel launch");
+}
+
 int run(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
     int rc = validate(h, q);
     if (rc != SL8_OK) return rc;
     std::lock_guard<std::mutex> lock(h->mu);
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(h, SL8_ERR_CUDA, "cudaSetDevice failed");
+    if (sl8::op_scaled(q.op) && h->forced_variant < 0 && q.M <= sl8::kFewRowsMax) return run_few(h, q, stream);
 
     int vid = h->forced_variant >= 0 ? h->forced_variant : pick_variant(h, q.op, q.out_dtype, q.M, q.N, q.K, q.flags);
     const VariantEntry* v = variant(vid);
@@ -276,7 +315,9 @@ int run(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
     if (rc != SL8_OK) return rc;
     // The last N tile is as wide as what is left of N (a multiple of 16): its MMAs run with that N and each CTA
     // brings tail / cta_group rows of B per k-block through a second map with a box of that height.
-    const int tail_cols = q.N % v->tn == 0 ? v->tn : q.N % v->tn;
+    // (kind::i8 of a CTA pair takes an N that is a multiple of 32: what the last 16 columns read of B past N is zeros, and their results are clipped)
+    int tail_cols = q.N % v->tn == 0 ? v->tn : q.N % v->tn;
+    if (q.op == kOpInt8 && v->cg == 2) tail_cols = (tail_cols + 31) / 32 * 32;
     map_bt = map_b;
     if (tail_cols != v->tn) {
         rc = encode_2d(h, &map_bt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.B, (unsigned long long)q.K, (unsigned long long)q.N,
@@ -318,8 +359,13 @@ int run(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
     const int k_last = q.K - (p.k_blocks - 1) * v->tk;
     p.last_kblock_mmas = (k_last + 31) / 32;
     p.tail_cols = tail_cols;
-    p.scale_a = q.scale_a;
-    p.scale_b = q.scale_b;
+    if (sl8::op_scaled(q.op)) {
+        p.row_scales = q.scale_a;
+        p.col_scales = q.scale_b;
+    } else {
+        p.scale_a = q.scale_a;
+        p.scale_b = q.scale_b;
+    }
     p.out_scale = q.out_scale;
     p.bias = q.bias;
     p.side = static_cast<const __nv_bfloat16*>(q.side);
@@ -504,6 +550,23 @@ SL8_API int sl8_fc2_residual_fp8(sl8_handle_t h, const void* A, int64_t lda, con
     q.scale_a = scale_a; q.scale_b = scale_b;
     q.bias = bias; q.side = residual; q.ld_side = ldr;
     q.D = D; q.ldd = ldd; q.M = M; q.N = N; q.K = K; q.flags = flags;
+    return run(h, q, static_cast<cudaStream_t>(stream));
+}
+
+SL8_API int sl8_linear_scaled(sl8_handle_t h, const void* A, int64_t lda, const void* B, int64_t ldb, int code_type,
+                              const float* scale_a, const float* scale_b, const void* bias, void* D, int64_t ldd, int64_t M,
+                              int N, int K, unsigned flags, sl8_stream_t stream) {
+    if (!h) return SL8_ERR_INVALID_VALUE;
+    if (code_type != SL8_CODE_E4M3 && code_type != SL8_CODE_INT8) return fail(h, SL8_ERR_INVALID_VALUE, "unknown code type");
+    if (flags & ~static_cast<unsigned>(SL8_FLAG_BIAS_F32 | SL8_FLAG_GELU)) return fail(h, SL8_ERR_INVALID_VALUE, "unknown flag bits");
+    Problem q = {};
+    q.op = code_type == SL8_CODE_INT8 ? kOpInt8 : kOpE4M3; q.out_dtype = SL8_OUT_BF16;
+    q.A = A; q.B = B; q.lda = lda; q.ldb = ldb;
+    q.scale_a = scale_a; q.scale_b = scale_b;
+    q.bias = bias;
+    q.D = D; q.ldd = ldd; q.M = M; q.N = N; q.K = K;
+    // (to the kernels the activation is the default, as in FC1)
+    q.flags = (flags & SL8_FLAG_BIAS_F32) | ((flags & SL8_FLAG_GELU) ? 0u : SL8_FLAG_NO_ACTIVATION);
     return run(h, q, static_cast<cudaStream_t>(stream));
 }
 

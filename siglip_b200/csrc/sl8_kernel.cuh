@@ -49,7 +49,10 @@
 
 namespace sl8 {
 
-enum : int { OP_PE = 0, OP_FC1 = 1, OP_FC2 = 2 };
+// OP_INT8, OP_E4M3: operands with a scale per row (sl8_linear_scaled), by the type of their codes.
+enum : int { OP_PE = 0, OP_FC1 = 1, OP_FC2 = 2, OP_INT8 = 3, OP_E4M3 = 4 };
+__host__ __device__ constexpr bool op_scaled(int op) { return op == OP_INT8 || op == OP_E4M3; }
+__host__ __device__ constexpr bool op_side(int op) { return op == OP_PE || op == OP_FC2; }       // a table or residual goes into the epilogue
 enum : int { OUT_BF16 = 0, OUT_E4M3 = 1 };
 // Measurement aids (skip one part of the kernel to time the rest).  They cost instructions in the
 // hot loops, so they exist only in a library built with -DSL8_DIAG.
@@ -117,6 +120,8 @@ struct KernelParams {
     const float* scale_a;
     const float* scale_b;
     const float* out_scale;
+    const float* row_scales;         // fp32 [M] and [N] (OP_INT8, OP_E4M3)
+    const float* col_scales;
     const void* bias;                // bf16 [N] or fp32 [N] (FLAG_BIAS_F32); may be null
     const __nv_bfloat16* side;       // table [period, N] (patch-embed) or residual [M, N] (FC2)
     long long ld_side;               // elements
@@ -131,7 +136,8 @@ struct KernelParams {
     long long* prof;                 // optional: PROF_SLOTS clock64 totals per CTA (null = tracing off)
 };
 
-template <int CG, int TN, int TK, int STAGES, int EPI_WARPS, int OUT, int NBUF>
+// VECS: fp32 vectors of a tile's columns that the epilogue keeps: the bias, and the columns' scales.
+template <int CG, int TN, int TK, int STAGES, int EPI_WARPS, int OUT, int NBUF, int VECS = 1>
 struct KernelTraits {
     static_assert(CG == 1 || CG == 2, "one CTA or a CTA pair per tile");
     static_assert(TN == 64 || TN == 128 || TN == 192 || TN == 256, "tile N");
@@ -167,8 +173,8 @@ struct KernelTraits {
     // fp32 bias of the current tile: one copy per epilogue warp in shared memory (broadcast reads) where that fits;
     // a configuration that needs every byte for the operand ring keeps it in registers instead (lane l holds the
     // bias of column l of each 32-column chunk) and broadcasts by warp shuffle.
-    static constexpr bool BIAS_IN_SMEM = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + EPI_WARPS * COLS_PER_WARP * 4 + 512 <= 232448;
-    static constexpr int BIAS_BYTES = BIAS_IN_SMEM ? EPI_WARPS * COLS_PER_WARP * 4 : 0;
+    static constexpr bool BIAS_IN_SMEM = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + VECS * EPI_WARPS * COLS_PER_WARP * 4 + 512 <= 232448;
+    static constexpr int BIAS_BYTES = BIAS_IN_SMEM ? VECS * EPI_WARPS * COLS_PER_WARP * 4 : 0;
     static constexpr int THREADS = (4 + EPI_WARPS) * 32;         // A producer, MMA, epilogue warps, side-data loader, B producer
     static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + STAGING_BYTES + BIAS_BYTES + BAR_BYTES;
     static_assert(STAGE_BYTES % 1024 == 0, "every operand tile must start on a swizzle-atom boundary");
@@ -455,6 +461,40 @@ __device__ __forceinline__ void epilogue_32_fc1(const float (&v)[32], const EpiC
     }
 }
 
+// Operands with a scale per row, COLS columns from FIRST of a 32-column chunk: acc * row scale * column scale + bias, GELU or not.
+// row_scale belongs to this lane's row; the columns' scales and biases come like the bias above.
+template <int OP, int FIRST, int COLS, bool BSM>
+__device__ __forceinline__ void epilogue_scaled(const float (&v)[32], const EpiCtx& e, float row_scale, const float* scale32, float sreg, const float* bias32,
+                                                float breg, uint32_t region, int piece0) {
+    const uint64_t row2 = pack_f32x2(row_scale, row_scale);
+    uint64_t g[COLS / 2];
+#pragma unroll
+    for (int i = 0; i < COLS / 4; i++) {
+        const float4 s = bias_quad<BSM>(scale32 + FIRST, sreg, FIRST, i);
+        const float4 b = bias_quad<BSM>(bias32 + FIRST, breg, FIRST, i);
+        float a[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)       // (a 32-bit sum beyond 2^24 is rounded here, by at most half a step of fp32)
+            a[j] = OP == OP_INT8 ? __int2float_rn(__float_as_int(v[FIRST + 4 * i + j])) : v[FIRST + 4 * i + j];
+        g[2 * i + 0] = fma_f32x2(mul_f32x2(pack_f32x2(a[0], a[1]), row2), pack_f32x2(s.x, s.y), pack_f32x2(b.x, b.y));
+        g[2 * i + 1] = fma_f32x2(mul_f32x2(pack_f32x2(a[2], a[3]), row2), pack_f32x2(s.z, s.w), pack_f32x2(b.z, b.w));
+    }
+    if (!(e.flags & FLAG_NO_ACTIVATION)) {                                           // warp-uniform
+#pragma unroll
+        for (int i = 0; i < COLS / 2; i++) g[i] = gelu_tanh_x2(g[i]);
+    }
+    uint32_t w[COLS / 2];
+#pragma unroll
+    for (int i = 0; i < COLS / 2; i++) {
+        float lo, hi;
+        unpack_f32x2(g[i], lo, hi);
+        w[i] = pack_bf16x2(lo, hi);
+    }
+#pragma unroll
+    for (int q = 0; q < COLS / 8; q++)
+        sts128(region + e.row_off + (((piece0 + FIRST / 8 + q) ^ e.swz) << 4), w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+}
+
 // Bias values of columns col0 + lane + 32 i (i < NB) as fp32; zero past N or without a bias.
 template <int NB>
 __device__ __forceinline__ void load_bias(float (&b)[NB], const void* bias, unsigned flags, int col0, int lane, int N) {
@@ -473,7 +513,7 @@ __global__ void __launch_bounds__((4 + EPI_WARPS) * 32, 1)
 sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ CUtensorMap map_bt, const __grid_constant__ CUtensorMap map_d,
                 const __grid_constant__ CUtensorMap map_s, const KernelParams p) {
-    using T = KernelTraits<CG, TN, TK, STAGES, EPI_WARPS, OUT, NBUF>;
+    using T = KernelTraits<CG, TN, TK, STAGES, EPI_WARPS, OUT, NBUF, op_scaled(OP) ? 2 : 1>;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_u32 = smem_u32(smem_raw);
@@ -543,7 +583,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     } else if (warp == 2 + EPI_WARPS) {
         if (elect_one()) {
             prefetch_tensormap(&map_d);
-            if constexpr (OP != OP_FC1) prefetch_tensormap(&map_s);
+            if constexpr (op_side(OP)) prefetch_tensormap(&map_s);
         }
     }
     __syncwarp();
@@ -696,8 +736,14 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         // stage's MMAs and read after them
         // (the blocking wait runs only if that look-ahead failed), and k-blocks are taken several per loop iteration.
         if (cta_rank == 0) {
-            const uint32_t idesc_full = make_idesc_e4m3_f32(T::TILE_M_CTA * CG, TN);
-            const uint32_t idesc_tail = make_idesc_e4m3_f32(T::TILE_M_CTA * CG, p.tail_cols);   // the last, narrower N tile
+            constexpr bool I8 = (OP == OP_INT8);
+            const uint32_t idesc_full = I8 ? make_idesc_i8_s32(T::TILE_M_CTA * CG, TN) : make_idesc_e4m3_f32(T::TILE_M_CTA * CG, TN);
+            const uint32_t idesc_tail = I8 ? make_idesc_i8_s32(T::TILE_M_CTA * CG, p.tail_cols)
+                                           : make_idesc_e4m3_f32(T::TILE_M_CTA * CG, p.tail_cols);   // the last, narrower N tile
+            const auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
+                if constexpr (I8) mma_i8<CG>(d, a, b, desc, accumulate);
+                else mma_f8<CG>(d, a, b, desc, accumulate);
+            };
             uint32_t idesc = idesc_full;
             // Descriptors differ between stages, atoms and K steps only in the 14-bit start-address
             // field: +2 there = 32 bytes = one K = 32 step inside the 128-byte row.
@@ -730,7 +776,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 for (int j = 0; j < 4 * T::KATOMS; j++) {
                     const uint32_t o = (j >> 2) * (T::A_ATOM_BYTES >> 4) + 2 * (j & 3);
                     const uint32_t ob = (j >> 2) * (T::B_ATOM_BYTES >> 4) + 2 * (j & 3);
-                    mma_f8<CG>(d_tmem, adesc + o, bdesc + ob, idesc, (j == 0 && fresh) ? 0u : 1u);
+                    mma(d_tmem, adesc + o, bdesc + ob, idesc, (j == 0 && fresh) ? 0u : 1u);
                 }
             };
             auto release_stage = [&](int st) {
@@ -772,7 +818,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                             for (int j = 0; j < 4 * T::KATOMS - 1; j++) {
                                 const uint32_t o = (j >> 2) * (T::A_ATOM_BYTES >> 4) + 2 * (j & 3);
                                 const uint32_t ob = (j >> 2) * (T::B_ATOM_BYTES >> 4) + 2 * (j & 3);
-                                if (j < n) mma_f8<CG>(d_tmem, adesc + o, bdesc + ob, idesc, (j == 0 && fresh) ? 0u : 1u);
+                                if (j < n) mma(d_tmem, adesc + o, bdesc + ob, idesc, (j == 0 && fresh) ? 0u : 1u);
                             }
                           }
                           release_stage(stage);
@@ -818,7 +864,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         for (int j = 0; j < p.last_kblock_mmas; j++) {
                             const uint32_t o = (j >> 2) * (T::A_ATOM_BYTES >> 4) + 2 * (j & 3);
                             const uint32_t ob = (j >> 2) * (T::B_ATOM_BYTES >> 4) + 2 * (j & 3);
-                            mma_f8<CG>(d_tmem, adesc + o, bdesc + ob, idesc, (kb | j) != 0 ? 1u : 0u);
+                            mma(d_tmem, adesc + o, bdesc + ob, idesc, (kb | j) != 0 ? 1u : 0u);
                         }
                       }
                     }
@@ -860,7 +906,8 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int col_begin = col_part * T::COLS_PER_WARP;
         constexpr int RPT = T::REGIONS_PER_TILE;
         constexpr bool HAS_BIAS = (OP != OP_PE);
-        constexpr bool HAS_SIDE = (OP != OP_FC1);
+        constexpr bool HAS_SIDE = op_side(OP);
+        constexpr bool SCALED = op_scaled(OP);
         static_assert(!HAS_SIDE || NBUF >= 2, "side data needs a buffer to land in while another is stored");
 
         EpiCtx e;
@@ -881,6 +928,28 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         float bnext[NB], bcur[NB];
 #pragma unroll
         for (int i = 0; i < NB; i++) bcur[i] = bnext[i] = 0.0f;
+        constexpr int NS = SCALED ? NB : 1;        // the columns' scales, likewise (behind all the biases in shared memory)
+        float* const scale_w = bias_w + EPI_WARPS * T::COLS_PER_WARP;
+        float snext[NS], scur[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) scur[i] = snext[i] = 0.0f;
+        // what the next tile's columns have goes to registers early, and from there to where this tile's was
+        const auto fetch_columns = [&](int tn) {
+            load_bias<NB>(bnext, p.bias, p.flags, tn * TN + col_begin, lane, p.N);
+            if constexpr (SCALED) load_bias<NS>(snext, p.col_scales, FLAG_BIAS_F32, tn * TN + col_begin, lane, p.N);
+        };
+        const auto keep_columns = [&]() {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                if constexpr (BSM) bias_w[lane + 32 * i] = bnext[i];
+                else bcur[i] = bnext[i];
+                if constexpr (SCALED) {
+                    if constexpr (BSM) scale_w[lane + 32 * i] = snext[i];
+                    else scur[i] = snext[i];
+                }
+            }
+            __syncwarp();
+        };
         bool ok = true;
         uint32_t seq = 0;                          // regions processed so far by this warp
         int acc = 0;
@@ -898,13 +967,8 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         e.inv_out = __frcp_rn(p.out_scale ? ld_f32(p.out_scale) : 1.0f);   // IEEE 1/x, as the CPU oracle computes it
         if constexpr (HAS_BIAS) {
             if (walk.tile < p.num_tiles) {
-                load_bias<NB>(bnext, p.bias, p.flags, walk.tn * TN + col_begin, lane, p.N);
-#pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    if constexpr (BSM) bias_w[lane + 32 * i] = bnext[i];
-                    else bcur[i] = bnext[i];
-                }
-                __syncwarp();
+                fetch_columns(walk.tn);
+                keep_columns();
             }
         }
         while (ok && walk.tile < p.num_tiles) {
@@ -917,7 +981,11 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             walk.next(p, num_clusters);
             const bool has_next = walk.tile < p.num_tiles;
             if constexpr (HAS_BIAS) {
-                if (has_next) load_bias<NB>(bnext, p.bias, p.flags, walk.tn * TN + col_begin, lane, p.N);
+                if (has_next) fetch_columns(walk.tn);
+            }
+            float row_scale = 0.0f;
+            if constexpr (SCALED) {
+                if (m_warp + lane < p.M) row_scale = ld_f32(p.row_scales + m_warp + lane);
             }
 
             long long t0 = prof_total ? clock64() : 0;       // once per tile: timed in the coarse mode too
@@ -985,8 +1053,22 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                                 for (int i = 1; i < NB; i++)
                                     if (i == r * T::CHUNKS_PER_REGION + ch) breg = bcur[i];
                             }
+                            float sreg = scur[0];
+                            if constexpr (SCALED && !BSM) {
+#pragma unroll
+                                for (int i = 1; i < NS; i++)
+                                    if (i == r * T::CHUNKS_PER_REGION + ch) sreg = scur[i];
+                            }
                             if (!SL8_DBG(p.flags, DBG_SKIP_MATH)) {
-                                if constexpr (OP == OP_FC1 && EPI_WARPS <= 8) {
+                                if constexpr (SCALED) {
+                                    const float* scale32 = scale_w + (c - col_begin);
+                                    if constexpr (EPI_WARPS <= 8) {
+                                        epilogue_scaled<OP, 0, 32, BSM>(v, e, row_scale, scale32, sreg, bias32, breg, region, piece0);
+                                    } else {
+                                        epilogue_scaled<OP, 0, 16, BSM>(v, e, row_scale, scale32, sreg, bias32, breg, region, piece0);
+                                        epilogue_scaled<OP, 16, 16, BSM>(v, e, row_scale, scale32, sreg, bias32, breg, region, piece0);
+                                    }
+                                } else if constexpr (OP == OP_FC1 && EPI_WARPS <= 8) {
                                     // (columns past N are computed on whatever the accumulator holds and clipped by the TMA store)
                                     epilogue_32_fc1<OUT, BSM>(v, e, bias32, breg, region, piece0);
                                 } else {
@@ -1033,12 +1115,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if constexpr (HAS_BIAS) {
                 if (has_next) {
                     __syncwarp();                        // every lane has finished reading this tile's bias
-#pragma unroll
-                    for (int i = 0; i < NB; i++) {
-                        if constexpr (BSM) bias_w[lane + 32 * i] = bnext[i];
-                        else bcur[i] = bnext[i];
-                    }
-                    __syncwarp();
+                    keep_columns();
                 }
             }
         }
@@ -1064,7 +1141,7 @@ sl8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         // expect; completion on the box's "landed" barrier.  One TMA load.  A positional table that holds
         // at least period + 127 rows (rows past the period repeating it) never needs anything else; with
         // an unpadded table the boxes that wrap around its end are copied row by row by the whole warp.
-        if constexpr (OP != OP_FC1) {
+        if constexpr (op_side(OP)) {
             constexpr int RPT = T::REGIONS_PER_TILE;
             constexpr int GROUPS = EPI_WARPS / 4;
             constexpr uint32_t BOX_BYTES = 4 * T::REGION_BYTES;

@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
+#include <initializer_list>
 
 #include "../../include/siglip_fp8.h"
 
@@ -96,15 +97,17 @@ inline bool codes(const at::Tensor& t) { return t.scalar_type() == at::kByte || 
 inline bool matrix(const at::Tensor& t) { return t.dim() == 2 && t.stride(1) == 1; }
 inline bool shaped(const at::Tensor& t, int64_t rows, int64_t cols) { return matrix(t) && t.size(0) == rows && t.size(1) == cols; }
 
-// A [M, K] and B [N, K], e4m3, K contiguous.
+// A [M, K] and B [N, K], e4m3 (or, where that is taken too, both int8), K contiguous.
 struct Gemm {
     const at::Tensor *A, *B;
     int64_t M = 0, N = 0, K = 0;
-    Gemm(Args& a) {
+    bool int8 = false;
+    Gemm(Args& a, bool int8_too = false) {
         A = a.tensor();
         B = a.ok ? a.tensor() : nullptr;
         if (!a.ok) return;
-        a.ok = codes(*A) && codes(*B) && matrix(*A) && matrix(*B) && A->size(1) == B->size(1) && B->size(0) <= INT_MAX && A->size(1) <= INT_MAX;
+        int8 = int8_too && A->scalar_type() == at::kChar && B->scalar_type() == at::kChar;
+        a.ok = (int8 || (codes(*A) && codes(*B))) && matrix(*A) && matrix(*B) && A->size(1) == B->size(1) && B->size(0) <= INT_MAX && A->size(1) <= INT_MAX;
         if (a.ok) { M = A->size(0); N = B->size(0); K = A->size(1); }
     }
 };
@@ -361,9 +364,123 @@ SL8_PY(layernorm_quantize) {
     END_HANDLE_TH_ERRORS
 }
 
+// New codes of the type that `kind` counts, or `given`; scales likewise.  Undefined codes: not the plain case.
+at::Tensor row_codes(const at::Tensor* given, const at::Tensor& x, int64_t rows, int64_t cols, long long kind) {
+    const at::ScalarType type = kind == 0 ? at::kChar : kind == 1 ? at::kFloat8_e4m3fn : at::kByte;
+    if (!given) return at::empty({rows, (cols + 127) / 128 * 128}, x.options().dtype(type)).narrow(1, 0, cols);
+    if (kind == 0 ? given->scalar_type() != at::kChar : !codes(*given)) return at::Tensor();
+    if (given->dim() != 2 || given->size(0) < rows || given->size(1) < cols || (given->stride(1) != 1 && given->size(1) != 1)) return at::Tensor();
+    return *given;
+}
+bool holds_scales(const at::Tensor& t, int64_t rows) { return t.scalar_type() == at::kFloat && t.numel() >= rows && (rows <= 1 || t.is_contiguous()); }
+
+PyObject* outputs(std::initializer_list<const at::Tensor*> all) {
+    PyObject* got[3];
+    Py_ssize_t n = 0;
+    for (const at::Tensor* t : all) {
+        if (!t->defined()) continue;
+        got[n] = THPVariable_Wrap(*t);
+        if (!got[n]) {
+            while (n > 0) Py_DECREF(got[--n]);
+            return nullptr;
+        }
+        n++;
+    }
+    if (n == 1) return got[0];
+    PyObject* tuple = PyTuple_New(n);
+    for (Py_ssize_t i = 0; i < n; i++) {
+        if (tuple) PyTuple_SET_ITEM(tuple, i, got[i]);
+        else Py_DECREF(got[i]);
+    }
+    return tuple;
+}
+
+// h, device, stream, x, out, scales, type of the codes (0 int8, 1 float8_e4m3fn, 2 uint8)  ->  (codes, scales)
+SL8_PY(quantize_rows) {
+    HANDLE_TH_ERRORS
+    Args a(args, count, 4);
+    if (!a.ok) Py_RETURN_NONE;
+    const at::Tensor* x = a.tensor();
+    bool has_out, has_scales;
+    const at::Tensor* given = a.ok ? a.optional(has_out) : nullptr;
+    const at::Tensor* given_scales = a.ok ? a.optional(has_scales) : nullptr;
+    const long long kind = a.ok ? a.integer() : 0;
+    if (!a.ok || !rows_of(*x)) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), cols = x->size(1);
+    if (given_scales && !holds_scales(*given_scales, rows)) Py_RETURN_NONE;
+    const at::Tensor out = row_codes(given, *x, rows, cols, kind);
+    if (!out.defined()) Py_RETURN_NONE;
+    const at::Tensor scales = given_scales ? *given_scales : at::empty({rows}, x->options().dtype(at::kFloat));
+    const int rc = unlocked(sl8_quantize_rows, a.h, x->const_data_ptr(), activation(*x), rows, static_cast<int>(cols), x->stride(0), kind == 0 ? SL8_CODE_INT8 : SL8_CODE_E4M3,
+                            out.mutable_data_ptr(), out.stride(0), static_cast<float*>(scales.mutable_data_ptr()), a.stream());
+    return rc != SL8_OK ? PyLong_FromLong(rc) : outputs({&out, &scales});
+    END_HANDLE_TH_ERRORS
+}
+
+// h, device, stream, x, gamma, residual, summed, scale, out, scales, eps, type of the codes (3: uint8, one scale for the tensor)
+//   ->  codes, with scales unless the tensor has one, and with summed if there is a residual
+SL8_PY(rmsnorm_quantize) {
+    HANDLE_TH_ERRORS
+    Args a(args, count, 9);
+    if (!a.ok) Py_RETURN_NONE;
+    const at::Tensor* x = a.tensor();
+    if (!a.ok || !rows_of(*x)) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), cols = x->size(1);
+    const float* gamma = a.floats(cols);
+    bool has_res, has_sum, has_out, has_scales;
+    const at::Tensor* residual = a.ok ? a.optional(has_res) : nullptr;
+    const at::Tensor* given_sum = a.ok ? a.optional(has_sum) : nullptr;
+    const float* scale = a.ok ? a.scale() : nullptr;
+    const at::Tensor* given = a.ok ? a.optional(has_out) : nullptr;
+    const at::Tensor* given_scales = a.ok ? a.optional(has_scales) : nullptr;
+    const double eps = a.ok ? a.real() : 0.0;
+    const long long kind = a.ok ? a.integer() : 0;
+    if (!a.ok || (given_sum && !residual)) Py_RETURN_NONE;
+    const auto like_x = [&](const at::Tensor* t) {
+        return !t || (t->scalar_type() == x->scalar_type() && t->dim() == 2 && t->size(0) == rows && t->size(1) == cols && (t->stride(1) == 1 || cols == 1));
+    };
+    if (!like_x(residual) || !like_x(given_sum) || (given_scales && !holds_scales(*given_scales, rows))) Py_RETURN_NONE;
+    const at::Tensor out = row_codes(given, *x, rows, cols, kind);
+    if (!out.defined()) Py_RETURN_NONE;
+    at::Tensor scales, sum;
+    if (kind != 3) scales = given_scales ? *given_scales : at::empty({rows}, x->options().dtype(at::kFloat));
+    if (residual) sum = given_sum ? *given_sum : at::empty({rows, cols}, x->options());
+    const int rc = unlocked(sl8_rmsnorm_quantize, a.h, x->const_data_ptr(), activation(*x), rows, static_cast<int>(cols), x->stride(0),
+                            residual ? residual->const_data_ptr() : nullptr, residual ? residual->stride(0) : int64_t{0},
+                            residual ? sum.mutable_data_ptr() : nullptr, residual ? sum.stride(0) : int64_t{0}, gamma, static_cast<float>(eps),
+                            kind == 0 ? SL8_CODE_INT8 : SL8_CODE_E4M3, scale, out.mutable_data_ptr(), out.stride(0),
+                            kind != 3 ? static_cast<float*>(scales.mutable_data_ptr()) : nullptr, a.stream());
+    return rc != SL8_OK ? PyLong_FromLong(rc) : outputs({&out, &scales, &sum});
+    END_HANDLE_TH_ERRORS
+}
+
+// h, device, stream, A, B, scale_a, scale_b, bias, out, flags
+SL8_PY(linear_scaled) {
+    HANDLE_TH_ERRORS
+    Args a(args, count, 7);
+    if (!a.ok) Py_RETURN_NONE;
+    Gemm g(a, true);
+    if (!a.ok) Py_RETURN_NONE;
+    const float *sa = a.floats(g.M), *sb = a.ok ? a.floats(g.N) : nullptr;
+    if (!a.ok || !sa || !sb) Py_RETURN_NONE;
+    bool has_bias, has_out;
+    const at::Tensor* bias = a.optional(has_bias);
+    const at::Tensor* given = a.ok ? a.optional(has_out) : nullptr;
+    unsigned flags = a.ok ? static_cast<unsigned>(a.integer()) : 0u;
+    const void* const b = bias_of(a, bias, g.N, flags);
+    if (!a.ok) Py_RETURN_NONE;
+    const at::Tensor out = output(a, given, *g.A, g.M, g.N, at::kBFloat16, false);
+    if (!a.ok) Py_RETURN_NONE;
+    const int rc = unlocked(sl8_linear_scaled, a.h, g.A->const_data_ptr(), g.A->stride(0), g.B->const_data_ptr(), g.B->stride(0), g.int8 ? SL8_CODE_INT8 : SL8_CODE_E4M3,
+                            sa, sb, b, out.mutable_data_ptr(), out.stride(0), g.M, static_cast<int>(g.N), static_cast<int>(g.K), flags, a.stream());
+    return result(rc, out);
+    END_HANDLE_TH_ERRORS
+}
+
 #define SL8_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SL8_METHOD(linear), SL8_METHOD(patch_embed), SL8_METHOD(fc2_residual), SL8_METHOD(mlp_chain),
                          SL8_METHOD(patchify_quantize), SL8_METHOD(amax_scale), SL8_METHOD(quantize_e4m3), SL8_METHOD(layernorm_quantize),
+                         SL8_METHOD(quantize_rows), SL8_METHOD(rmsnorm_quantize), SL8_METHOD(linear_scaled),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "sl8_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,5 +1,5 @@
-// sl8_variant.cu -- instantiates the four kernels (patch-embed, FC1 -> bf16, FC1 -> e4m3,
-// FC2) of ONE tile configuration and exports its table entry.  Compiled once per entry of
+// sl8_variant.cu -- instantiates the kernels (patch-embed, FC1 -> bf16, FC1 -> e4m3,
+// FC2, and operands with a scale per row where the variant serves them) of ONE tile configuration and exports its table entry.  Compiled once per entry of
 // SL8_VARIANT_LIST with -DSL8_VARIANT_ID=<id>, so the configurations build in parallel.
 #include <type_traits>
 
@@ -15,7 +15,7 @@ namespace {
 template <int CG, int TN, int TK, int STAGES, int EW, int OP, int OUT, int NBUF>
 cudaError_t launch_one(const CUtensorMap* map_a, const CUtensorMap* map_b, const CUtensorMap* map_bt, const CUtensorMap* map_d,
                        const CUtensorMap* map_s, const KernelParams* params, int grid, cudaStream_t stream) {
-    using T = KernelTraits<CG, TN, TK, STAGES, EW, OUT, NBUF>;
+    using T = KernelTraits<CG, TN, TK, STAGES, EW, OUT, NBUF, op_scaled(OP) ? 2 : 1>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
     cfg.blockDim = dim3(T::THREADS, 1, 1);
@@ -51,13 +51,17 @@ const VariantEntry* make_entry() {
     using T16 = KernelTraits<CG, TN, TK, STAGES, EW, OUT_BF16, NBUF>;
     constexpr bool E4 = (TN / (EW / 4)) % 64 == 0;   // an e4m3 staging region is 128 or 64 columns wide
     using T8 = std::conditional_t<E4, KernelTraits<CG, TN, TK, STAGES, EW, E4 ? OUT_E4M3 : OUT_BF16, NBUF>, T16>;
+    constexpr bool ROWS = serves_scaled(ID);
+    using TS = KernelTraits<CG, TN, TK, STAGES, EW, OUT_BF16, NBUF, 2>;
     static const VariantEntry e = {
         ID, CG, TN, TK, STAGES, EW, NBUF, T16::A_BOX_ROWS, T16::THREADS,
-        {T16::SMEM_BYTES, T16::SMEM_BYTES, T8::SMEM_BYTES, T16::SMEM_BYTES},
+        {T16::SMEM_BYTES, T16::SMEM_BYTES, T8::SMEM_BYTES, T16::SMEM_BYTES, TS::SMEM_BYTES, TS::SMEM_BYTES},
         {Slot<CG, TN, TK, STAGES, EW, OP_PE, OUT_BF16, NBUF, SIDE>::kernel(), Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_BF16, NBUF, true>::kernel(),
-         Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_E4M3, NBUF, E4>::kernel(), Slot<CG, TN, TK, STAGES, EW, OP_FC2, OUT_BF16, NBUF, SIDE>::kernel()},
+         Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_E4M3, NBUF, E4>::kernel(), Slot<CG, TN, TK, STAGES, EW, OP_FC2, OUT_BF16, NBUF, SIDE>::kernel(),
+         Slot<CG, TN, TK, STAGES, EW, OP_INT8, OUT_BF16, NBUF, ROWS>::kernel(), Slot<CG, TN, TK, STAGES, EW, OP_E4M3, OUT_BF16, NBUF, ROWS>::kernel()},
         {Slot<CG, TN, TK, STAGES, EW, OP_PE, OUT_BF16, NBUF, SIDE>::launcher(), Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_BF16, NBUF, true>::launcher(),
-         Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_E4M3, NBUF, E4>::launcher(), Slot<CG, TN, TK, STAGES, EW, OP_FC2, OUT_BF16, NBUF, SIDE>::launcher()}};
+         Slot<CG, TN, TK, STAGES, EW, OP_FC1, OUT_E4M3, NBUF, E4>::launcher(), Slot<CG, TN, TK, STAGES, EW, OP_FC2, OUT_BF16, NBUF, SIDE>::launcher(),
+         Slot<CG, TN, TK, STAGES, EW, OP_INT8, OUT_BF16, NBUF, ROWS>::launcher(), Slot<CG, TN, TK, STAGES, EW, OP_E4M3, OUT_BF16, NBUF, ROWS>::launcher()}};
     return &e;
 }
 

@@ -47,8 +47,13 @@
 
 namespace sl8 {
 
-// Kernel slots of a variant: layer x output type.
-enum : int { K_PE = 0, K_FC1_BF16 = 1, K_FC1_E4M3 = 2, K_FC2 = 3, K_COUNT = 4 };
+// Kernel slots of a variant: layer x output type; operands with a scale per row, by the type of their codes.
+enum : int { K_PE = 0, K_FC1_BF16 = 1, K_FC1_E4M3 = 2, K_FC2 = 3, K_INT8 = 4, K_E4M3 = 5, K_COUNT = 6 };
+
+// The variants that are compiled for operands with a scale per row.
+constexpr bool serves_scaled(int id) {
+    return id == 1 || id == 2 || id == 3 || id == 14 || id == 15 || id == 18 || id == 19 || id == 20 || id == 21;
+}
 
 // map_bt: B with a box as tall as one CTA's share of the last, narrower N tile (== map_b when N % tile N == 0).
 typedef cudaError_t (*launch_fn)(const CUtensorMap* map_a, const CUtensorMap* map_b, const CUtensorMap* map_bt,

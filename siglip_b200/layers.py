@@ -28,6 +28,11 @@ def _is_fp8(t: torch.Tensor) -> bool:
     return t.dtype in (torch.uint8, torch.float8_e4m3fn)
 
 
+def _code_type(dtype: torch.dtype) -> Optional[int]:
+    """SL8_CODE_* of a tensor of codes with a scale for each row."""
+    return _l.SL8_CODE_INT8 if dtype == torch.int8 else _l.SL8_CODE_E4M3 if dtype in (torch.uint8, torch.float8_e4m3fn) else None
+
+
 class Engine:
     """One handle of libsiglip_fp8.so (``sl8_create``) on CUDA device ``device``."""
 
@@ -92,6 +97,9 @@ class Engine:
     def _operands(self, A: torch.Tensor, B: torch.Tensor):
         if not (_is_fp8(A) and _is_fp8(B)):
             raise TypeError("A and B must be float8_e4m3fn or uint8 (raw e4m3 codes)")
+        return self._matrices(A, B)
+
+    def _matrices(self, A: torch.Tensor, B: torch.Tensor):
         if A.dim() != 2 or B.dim() != 2 or A.stride(1) != 1 or B.stride(1) != 1:
             raise ValueError("A [M, K] and B [N, K] must be 2-D with K contiguous")
         if not (A.is_cuda and B.is_cuda):
@@ -363,14 +371,15 @@ class Engine:
             raise ValueError("x must be [rows, cols] with the columns contiguous")
         return x.shape
 
-    def _codes_into(self, out: torch.Tensor, rows: int, cols: int) -> None:
+    def _codes_into(self, out: torch.Tensor, rows: int, cols: int, types: Optional[tuple] = None) -> None:
         """A caller-supplied buffer for [rows, cols] codes: one code after the other in a row, and at least that large (the
         library knows its address and row pitch, not where it ends).  A pitch below a row's codes it refuses itself."""
         if out.dim() > 0 and out.stride(0) < cols:
             return
         self._readable("out", out)
-        if out.dtype not in self._E4M3_TYPES:
-            raise TypeError(f"out has dtype {out.dtype}; codes are float8_e4m3fn or uint8")
+        types = self._E4M3_TYPES if types is None else types
+        if out.dtype not in types:
+            raise TypeError(f"out has dtype {out.dtype}; codes are {' or '.join(str(t).removeprefix('torch.') for t in types)}")
         if out.dim() != 2 or out.shape[0] < rows or out.shape[1] < cols or (out.stride(1) != 1 and out.shape[1] != 1):
             raise ValueError(f"out [{', '.join(map(str, out.shape))}] must hold [{rows}, {cols}] codes, columns contiguous")
 
@@ -456,6 +465,129 @@ class Engine:
             self._h, x.data_ptr(), self._dt(x), rows, cols, x.stride(0), _ptr(gamma), _ptr(beta), float(eps), _ptr(scale),
             out.data_ptr(), out.stride(0), self._stream(stream)))
         return out
+
+    # ------------------------------------------------------------------ 8-bit operands with a scale for each row
+    _ROW_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1, torch.uint8: 2}       # as the extension module counts them
+
+    def _row_codes(self, x, rows: int, cols: int, dtype, out) -> torch.Tensor:
+        """`out`, or new codes of `dtype` on rows of 128-byte lines."""
+        if dtype not in self._ROW_TYPES:
+            raise TypeError("codes with a scale for each row are int8, float8_e4m3fn or uint8 (raw e4m3 codes)")
+        if out is None:
+            self._on_device("x", x)
+            return torch.empty((rows, (cols + 127) // 128 * 128), dtype=torch.uint8, device=x.device).view(dtype)[:, :cols]
+        self._readable("x", x)
+        self._codes_into(out, rows, cols, (torch.int8,) if dtype == torch.int8 else self._E4M3_TYPES)
+        if _code_type(out.dtype) != _code_type(dtype):        # (a pitch that the library refuses is not looked at above)
+            raise TypeError(f"dtype {dtype} contradicts out.dtype {out.dtype}")
+        return out
+
+    def _row_scales(self, scales, rows: int, device) -> torch.Tensor:
+        """`scales`, or a new fp32 [rows]."""
+        if scales is None:
+            return torch.empty((rows,), dtype=torch.float32, device=device)
+        self._floats("scales", scales, rows)
+        self._readable("scales", scales)
+        return scales
+
+    def _stream_of(self, x, residual, summed, rows: int, cols: int):
+        """The residual and where its sum with x goes: both None, or both matrices of x's shape and type."""
+        if residual is None:
+            if summed is not None:
+                raise ValueError("summed is what the residual's addition writes: there is no residual")
+            return None
+        for name, t in (("residual", residual), ("summed", summed)):
+            if t is None:
+                continue
+            if t.dtype != x.dtype or tuple(t.shape) != (rows, cols) or (t.stride(1) != 1 and cols != 1):
+                raise ValueError(f"{name} must be {x.dtype} [{rows}, {cols}] with the columns contiguous, like x")
+            self._readable(name, t)
+        if summed is None:
+            self._on_device("x", x)
+            summed = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        return summed
+
+    def quantize_rows(self, x, dtype=torch.int8, *, out=None, scales=None, stream=None):
+        """(codes, scales): x in 8 bits with a scale for each row, max |row| / 127 (int8) or / 448 (float8_e4m3fn; uint8: the
+        raw codes).  The operands of :meth:`linear_scaled`: an activation [M, K] or weights [N, K].  New codes lie on rows of
+        128-byte lines; scales are fp32 [rows].  A row with an infinity or NaN gets the scale NaN."""
+        kind = self._ROW_TYPES.get(dtype)
+        if kind is not None:
+            r = self._native.quantize_rows(self._handle, self.device, None if stream is None else self._stream(stream), x, out, scales, kind)
+            if r is not None:
+                return self._done(r)
+        rows, cols = self._rows(x)
+        out = self._row_codes(x, rows, cols, dtype, out)
+        scales = self._row_scales(scales, rows, out.device)
+        self._check(self._lib.sl8_quantize_rows(self._h, x.data_ptr(), self._dt(x), rows, cols, x.stride(0), _code_type(out.dtype),
+                                                out.data_ptr(), out.stride(0), scales.data_ptr(), self._stream(stream)))
+        return out, scales
+
+    def rmsnorm_quantize_rows(self, x, gamma=None, eps: float = 1e-6, dtype=torch.int8, *, residual=None, summed=None, out=None,
+                              scales=None, stream=None):
+        """(codes, scales) of h * rsqrt(mean(h^2) + eps) * gamma, quantised like :meth:`quantize_rows`.  h is x, or x + residual
+        with a residual of x's shape and type: then (codes, scales, summed), where ``summed`` (x or the residual itself, if they
+        need not be kept; new when None) holds h, the new residual stream.  gamma fp32 [cols]."""
+        kind = self._ROW_TYPES.get(dtype)
+        if kind is not None:
+            r = self._native.rmsnorm_quantize(self._handle, self.device, None if stream is None else self._stream(stream),
+                                              x, gamma, residual, summed, None, out, scales, eps, kind)
+            if r is not None:
+                return self._done(r)
+        rows, cols = self._rows(x)
+        self._floats("gamma", gamma, cols)
+        self._readable("gamma", gamma)
+        out = self._row_codes(x, rows, cols, dtype, out)
+        scales = self._row_scales(scales, rows, out.device)
+        return self._rmsnorm(x, rows, cols, gamma, eps, residual, summed, None, out, scales, stream)
+
+    def rmsnorm_quantize(self, x, gamma=None, eps: float = 1e-6, scale=None, *, residual=None, summed=None, out=None, stream=None):
+        """e4m3 codes (uint8) of h * rsqrt(mean(h^2) + eps) * gamma / scale, one scale for the tensor: the A operand of the layers
+        above, as :meth:`layernorm_quantize` makes it.  With a residual (codes, summed), see :meth:`rmsnorm_quantize_rows`."""
+        r = self._native.rmsnorm_quantize(self._handle, self.device, None if stream is None else self._stream(stream),
+                                          x, gamma, residual, summed, scale, out, None, eps, 3)
+        if r is not None:
+            return self._done(r)
+        rows, cols = self._rows(x)
+        for name, t, n in (("gamma", gamma, cols), ("scale", scale, 1)):
+            self._floats(name, t, n)
+            self._readable(name, t)
+        out = self._row_codes(x, rows, cols, torch.uint8, out)
+        return self._rmsnorm(x, rows, cols, gamma, eps, residual, summed, scale, out, None, stream)
+
+    def _rmsnorm(self, x, rows, cols, gamma, eps, residual, summed, scale, out, scales, stream):
+        summed = self._stream_of(x, residual, summed, rows, cols)
+        self._check(self._lib.sl8_rmsnorm_quantize(
+            self._h, x.data_ptr(), self._dt(x), rows, cols, x.stride(0), _ptr(residual), 0 if residual is None else residual.stride(0),
+            _ptr(summed), 0 if summed is None else summed.stride(0), _ptr(gamma), float(eps), _code_type(out.dtype), _ptr(scale),
+            out.data_ptr(), out.stride(0), _ptr(scales), self._stream(stream)))
+        got = tuple(t for t in (out, scales, summed) if t is not None)
+        return got if len(got) > 1 else out
+
+    def linear_scaled(self, A, B, scale_a, scale_b, bias=None, *, out=None, flags: int = 0, stream=None) -> torch.Tensor:
+        """D = bf16(f(A.B^T * scale_a[:, None] * scale_b + bias)): A [M, K] and B [N, K] both int8 or both e4m3 codes with a scale
+        for each row (fp32 [M], [N]: a token, an output channel), f the identity or, with SL8_FLAG_GELU, GELU(tanh).  int8 products are
+        summed exactly."""
+        r = self._native.linear_scaled(self._handle, self.device, None if stream is None else self._stream(stream),
+                                       A, B, scale_a, scale_b, bias, out, flags)
+        if r is not None:
+            return self._done(r)
+        code = _code_type(A.dtype)
+        if code is None or _code_type(B.dtype) != code:
+            raise TypeError("A and B must both be int8, or both float8_e4m3fn or uint8 (raw e4m3 codes)")
+        M, N, K = self._matrices(A, B)
+        flags = self._bias_flags(flags, ("bias", bias, N))
+        for name, t, n in (("scale_a", scale_a, M), ("scale_b", scale_b, N)):
+            if t is None:
+                raise ValueError(f"{name} is required: a scale for each row of {name[-1].upper()}")
+            self._on_device(name, t)
+            self._floats(name, t, n)
+        self._on_device("bias", bias)
+        D = self._new_out(M, N, torch.bfloat16, A.device) if out is None else self._check_out(out, M, N, (torch.bfloat16,))
+        self._check(self._lib.sl8_linear_scaled(
+            self._h, A.data_ptr(), A.stride(0), B.data_ptr(), B.stride(0), code, scale_a.data_ptr(), scale_b.data_ptr(), _ptr(bias),
+            D.data_ptr(), D.stride(0), M, N, K, int(flags), self._stream(stream)))
+        return D
 
     # ------------------------------------------------------------------ host operands
     def patch_embed_host(self, A, B, table, out, *, period=None, scale_a=1.0, scale_b=1.0, row_phase=0, flags=0):

@@ -27,7 +27,8 @@ SL8_ERR_NO_DEVICE = -7
 
 SL8_OUT_BF16, SL8_OUT_E4M3 = 0, 1
 SL8_OP_PATCH_EMBED, SL8_OP_FC1_GELU, SL8_OP_FC2_RESIDUAL = 0, 1, 2
-SL8_FLAG_NONE, SL8_FLAG_BIAS_F32, SL8_FLAG_PE_F32_ADD, SL8_FLAG_NO_ACTIVATION, SL8_FLAG_GELU_HW_TANH = 0, 1, 2, 4, 8
+SL8_FLAG_NONE, SL8_FLAG_BIAS_F32, SL8_FLAG_PE_F32_ADD, SL8_FLAG_NO_ACTIVATION, SL8_FLAG_GELU_HW_TANH, SL8_FLAG_GELU = 0, 1, 2, 4, 8, 16
+SL8_CODE_E4M3, SL8_CODE_INT8 = 0, 1
 SL8_DT_F32, SL8_DT_BF16 = 0, 1
 
 _ERR_NAMES = {
@@ -71,6 +72,9 @@ SIGNATURES = {
     "sl8_amax_scale": (_I, [_P, _P, _I, _I64, _I, _I64, _P, _P, _P]),
     "sl8_quantize_e4m3": (_I, [_P, _P, _I, _I64, _I, _I64, _P, _P, _I64, _P]),
     "sl8_layernorm_quantize_e4m3": (_I, [_P, _P, _I, _I64, _I, _I64, _P, _P, _F, _P, _P, _I64, _P]),
+    "sl8_quantize_rows": (_I, [_P, _P, _I, _I64, _I, _I64, _I, _P, _I64, _P, _P]),
+    "sl8_rmsnorm_quantize": (_I, [_P, _P, _I, _I64, _I, _I64, _P, _I64, _P, _I64, _P, _F, _I, _P, _P, _I64, _P, _P]),
+    "sl8_linear_scaled": (_I, [_P, _P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I64, _I64, _I, _I, _U, _P]),
     "sl8_patch_embed_fp8_host": (_I, [_P, _P, _I64, _P, _I64, _F, _F, _P, _I64, _I, _I, _I, _P, _I64, _I64, _I, _I, _U]),
     "sl8_fc1_gelu_fp8_host": (_I, [_P, _P, _I64, _P, _I64, _F, _F, _P, _P, _I64, _I, _F, _I64, _I, _I, _U]),
     "sl8_fc2_residual_fp8_host": (_I, [_P, _P, _I64, _P, _I64, _F, _F, _P, _P, _I64, _P, _I64, _I64, _I, _I, _U]),
