@@ -907,7 +907,7 @@ SL8_API int sl8_device_status(sl8_handle_t h, sl8_stream_t stream, unsigned deta
     static const char* names[] = {"", "producer waiting for a free stage", "MMA thread waiting for operands",
                                   "MMA thread waiting for a free accumulator", "epilogue waiting for an accumulator",
                                   "epilogue waiting for table / residual data",
-                                  "table / residual loader waiting for a free staging box"};
+                                  "table / residual loader waiting for a free staging box", "row waiting for its elements"};
     constexpr unsigned kNames = sizeof names / sizeof names[0];
     snprintf(buf, sizeof buf, "device wait expired: %s (index %u, tile %u, block %u)", st[0] < kNames ? names[st[0]] : "?", st[1],
              st[2], st[3]);

@@ -82,7 +82,8 @@ enum : uint32_t {
     ST_MMA_TMEM_EMPTY_WAIT = 3,
     ST_EPI_TMEM_FULL_WAIT = 4,
     ST_EPI_SIDE_WAIT = 5,
-    ST_SIDE_LOADER_WAIT = 6
+    ST_SIDE_LOADER_WAIT = 6,
+    ST_ROW_WAIT = 7
 };
 
 // Tracing slots written per CTA when KernelParams::prof is set (cycles, clock64).

@@ -20,9 +20,12 @@ struct RowArgs {
     long long rows;
     int cols;
     int int8;                                    // codes: int8, else e4m3
+    uint32_t* status;                            // bounded waits, as in the GEMMs
+    unsigned wait_budget_us;
+    int drop;                                    // test aid: the copy of row 1 is never issued
 };
 
-// ---- eight consecutive elements as they lie in memory, and their values
+// ---- eight elements of a row as they lie in memory, and their values
 template <typename T>
 struct Eight {
     uint32_t w[2 * sizeof(T)];
@@ -32,9 +35,11 @@ __device__ __forceinline__ uint16_t ld_u16(const void* p) {
     asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
     return v;
 }
-// `have` of them; VEC: all eight, from a 16-byte boundary.
+// VEC: eight in a row from a 16-byte boundary.  Otherwise every 32nd, so that the lanes of a warp read consecutive elements: a warp has
+// the same 256 of a row either way.  `left`: elements from the first of the eight to the row's end; the ones beyond are zero (the
+// last of the row is read in their place: no load waits for a condition on another).
 template <bool VEC, typename T>
-__device__ __forceinline__ void fetch(Eight<T>& e, const T* p, int have) {
+__device__ __forceinline__ void fetch(Eight<T>& e, const T* p, int left) {
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++) {
@@ -42,15 +47,21 @@ __device__ __forceinline__ void fetch(Eight<T>& e, const T* p, int have) {
             e.w[4 * i] = q.x; e.w[4 * i + 1] = q.y; e.w[4 * i + 2] = q.z; e.w[4 * i + 3] = q.w;
         }
     } else {
+        const auto put = [&](int i, const T* at, bool inside) {
+            uint32_t b;
+            if constexpr (sizeof(T) == 4) b = __float_as_uint(sl8::ld_f32(at));
+            else b = ld_u16(at);
+            if (!inside) b = 0u;
+            if constexpr (sizeof(T) == 4) e.w[i] = b;
+            else if (i & 1) e.w[i / 2] |= b << 16;
+            else e.w[i / 2] = b;
+        };
+        if (left > 224) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if constexpr (sizeof(T) == 4) {
-                e.w[i] = i < have ? __float_as_uint(sl8::ld_f32(p + i)) : 0u;
-            } else {
-                const uint32_t b = i < have ? ld_u16(p + i) : 0u;
-                if (i & 1) e.w[i / 2] |= b << 16;
-                else e.w[i / 2] = b;
-            }
+            for (int i = 0; i < 8; i++) put(i, p + 32 * i, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) put(i, p + min(32 * i, left - 1), 32 * i < left);
         }
     }
 }
@@ -60,57 +71,85 @@ __device__ __forceinline__ float value(const Eight<T>& e, int i) {
     else return (i & 1) ? sl8::bf16_hi_f32(e.w[i / 2]) : sl8::bf16_lo_f32(e.w[i / 2]);
 }
 template <bool VEC, typename T>
-__device__ __forceinline__ void put_sum(T* p, const float (&v)[8], int have) {
-    if constexpr (sizeof(T) == 4) {
-        if constexpr (VEC) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < have) p[i] = v[i];
-        }
-    } else {
-        if constexpr (VEC) {
-            *reinterpret_cast<uint4*>(p) = make_uint4(sl8::pack_bf16x2(v[0], v[1]), sl8::pack_bf16x2(v[2], v[3]),
-                                                      sl8::pack_bf16x2(v[4], v[5]), sl8::pack_bf16x2(v[6], v[7]));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < have) p[i] = __float2bfloat16_rn(v[i]);
-        }
-    }
-}
-
-// Four int8 codes: y * inv + 1.5 * 2^23 leaves round-to-nearest-even(y * inv) in the low byte (|y * inv| <= 127).
-__device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d, float inv) {
-    constexpr float M = 12582912.0f;
-    const uint32_t p = __float_as_uint(fmaf(a, inv, M)), q = __float_as_uint(fmaf(b, inv, M));
-    const uint32_t r = __float_as_uint(fmaf(c, inv, M)), s = __float_as_uint(fmaf(d, inv, M));
-    return __byte_perm(__byte_perm(p, q, 0x0040), __byte_perm(r, s, 0x0040), 0x5410);
-}
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
-    return static_cast<uint32_t>(sl8::pack_e4m3x2(a * inv, b * inv)) | (static_cast<uint32_t>(sl8::pack_e4m3x2(c * inv, d * inv)) << 16);
-}
-template <bool VEC>
-__device__ __forceinline__ void put_codes(uint8_t* p, const float (&y)[8], float inv, bool int8, int have) {
-    const uint32_t lo = int8 ? int8x4(y[0], y[1], y[2], y[3], inv) : e4m3x4(y[0], y[1], y[2], y[3], inv);
-    const uint32_t hi = int8 ? int8x4(y[4], y[5], y[6], y[7], inv) : e4m3x4(y[4], y[5], y[6], y[7], inv);
-    if constexpr (VEC) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+__device__ __forceinline__ void put_sum(T* p, const float (&v)[8], int left) {
+    if constexpr (VEC && sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(sl8::pack_bf16x2(v[0], v[1]), sl8::pack_bf16x2(v[2], v[3]),
+                                                  sl8::pack_bf16x2(v[4], v[5]), sl8::pack_bf16x2(v[6], v[7]));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            if (i < have) p[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            if (32 * i < left) {
+                if constexpr (sizeof(T) == 4) p[32 * i] = v[i];
+                else p[32 * i] = __float2bfloat16_rn(v[i]);
+            }
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ void times_gamma(float (&v)[8], const float* gamma, int left) {      // gamma: shared memory
+    if constexpr (VEC) {
+        const float4 lo = reinterpret_cast<const float4*>(gamma)[0], hi = reinterpret_cast<const float4*>(gamma)[1];
+        v[0] *= lo.x; v[1] *= lo.y; v[2] *= lo.z; v[3] *= lo.w;
+        v[4] *= hi.x; v[5] *= hi.y; v[6] *= hi.z; v[7] *= hi.w;
+    } else {
+        if (left > 224) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= gamma[32 * i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (32 * i < left) v[i] *= gamma[32 * i];
+        }
     }
 }
 
-// |v| as an integer: ordered like the numbers, infinity above them and NaN above that, so that none gets lost in a maximum.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// v * k + 1.5 * 2^23, one rounding, leaves round-to-nearest-even(v * k) in the low byte (|v * k| < 127.5).
+__device__ __forceinline__ uint32_t int8_of(float v, float k) { return __float_as_uint(fmaf(v, k, 12582912.0f)); }
+__device__ __forceinline__ uint32_t int8x4(const float* v, float k) {
+    return __byte_perm(__byte_perm(int8_of(v[0], k), int8_of(v[1], k), 0x0040), __byte_perm(int8_of(v[2], k), int8_of(v[3], k), 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t e4m3x4(const float* v, float k) {
+    return static_cast<uint32_t>(sl8::pack_e4m3x2(v[0] * k, v[1] * k)) | (static_cast<uint32_t>(sl8::pack_e4m3x2(v[2] * k, v[3] * k)) << 16);
+}
+template <bool VEC>
+__device__ __forceinline__ void put_codes(uint8_t* p, const float (&v)[8], float k, bool int8, int left) {
+    if constexpr (VEC) {
+        *reinterpret_cast<uint2*>(p) = int8 ? make_uint2(int8x4(v, k), int8x4(v + 4, k)) : make_uint2(e4m3x4(v, k), e4m3x4(v + 4, k));
+    } else {
+        uint32_t code[8];
+        if (int8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) code[i] = int8_of(v[i], k);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                code[i] = sl8::pack_e4m3x2(v[i] * k, v[i + 1] * k);
+                code[i + 1] = code[i] >> 8;
+            }
+        }
+        if (left > 224) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[32 * i] = static_cast<uint8_t>(code[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (32 * i < left) p[32 * i] = static_cast<uint8_t>(code[i]);
+        }
+    }
+}
+
+// The largest of m and eight magnitudes; a NaN among them is the largest.
+__device__ __forceinline__ float largest_of(float m, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+    return m;
+}
 
 struct Stats {
     float squares;        // sum of h^2
-    uint32_t largest;     // magnitude of the largest h * gamma
+    float largest;        // largest |h * gamma|
 };
 template <bool NORM>
 __device__ __forceinline__ Stats reduce_warp(Stats s) {
@@ -118,151 +157,345 @@ __device__ __forceinline__ Stats reduce_warp(Stats s) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s.squares += __shfl_xor_sync(0xffffffffu, s.squares, o);
     }
-    s.largest = __reduce_max_sync(0xffffffffu, s.largest);
+    s.largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s.largest)));     // (as integers: ordered like the numbers, NaN above infinity)
     return s;
 }
-// Over the G threads of a row; `turn` counts the calls (the rows of a block use two sets of partial results in turn, so one barrier does).
-template <bool NORM, int G>
-__device__ __forceinline__ Stats reduce(Stats s, int turn) {
+// Over the threads of a block; `turn` counts the calls (they use two sets of partial results in turn, so one barrier does).
+template <bool NORM>
+__device__ __forceinline__ Stats reduce_block(Stats s, int turn) {
+    __shared__ Stats part[2][32];
     s = reduce_warp<NORM>(s);
-    if constexpr (G > 32) {
-        __shared__ Stats part[2][G / 32];
-        if ((threadIdx.x & 31) == 0) part[turn & 1][threadIdx.x >> 5] = s;
-        __syncthreads();
-        s = part[turn & 1][0];
-#pragma unroll
-        for (int i = 1; i < G / 32; i++) {
-            const Stats o = part[turn & 1][i];
-            s.squares += o.squares;
-            s.largest = max(s.largest, o.largest);
-        }
-    }
-    return s;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) part[turn & 1][threadIdx.x >> 5] = s;
+    __syncthreads();
+    return reduce_warp<NORM>(lane < static_cast<int>(blockDim.x >> 5) ? part[turn & 1][lane] : Stats{0.0f, 0.0f});
 }
 
-// What a row's codes are multiples of, and its reciprocal.
+constexpr float kInfinity = __builtin_huge_valf(), kSmallest = 1.17549435e-38f /* 2^-126 */, kLargest = 3.40282347e38f;
+
+// A row's codes are round(v * k), v = h * gamma (times rstd first where `small`).
 struct Scaling {
-    float rstd, scale, inv;
+    float rstd, scale, k;
+    bool small;
 };
 template <bool NORM>
-__device__ __forceinline__ Scaling scaling(const RowArgs& a, const Stats& s, float inv_n, float given_inv) {
+__device__ __forceinline__ Scaling scaling(const RowArgs& a, const Stats& s, float given) {
     Scaling r;
+    const float nan = __int_as_float(0x7FC00000);
     // a sum of squares that is no number (an infinity or NaN among the elements, or squares beyond fp32): nothing that comes out is one
-    r.rstd = !NORM ? 1.0f : s.squares < __int_as_float(0x7F800000) ? rsqrtf(fmaf(s.squares, inv_n, a.eps)) : __int_as_float(0x7FC00000);
-    r.scale = 0.0f;
-    r.inv = given_inv;
-    if (a.row_scales) {
-        // rounding is monotonic: the largest |h * gamma| times rstd is the largest |h * gamma * rstd|
-        const float largest = __uint_as_float(s.largest) * r.rstd;
-        if (largest == 0.0f) r.scale = 1.0f;
-        else if (largest < __int_as_float(0x7F800000)) r.scale = fmaxf(__fdiv_rn(largest, a.int8 ? 127.0f : 448.0f), 1.17549435e-38f);
-        else r.scale = __int_as_float(0x7FC00000);
-        r.inv = __frcp_rn(r.scale);
+    r.rstd = !NORM ? 1.0f : s.squares < kInfinity ? __frsqrt_rn(__fdiv_rn(s.squares, static_cast<float>(a.cols)) + a.eps) : nan;
+    r.small = false;
+    if (!a.row_scales) {
+        r.scale = 0.0f;
+        r.k = __fdiv_rn(r.rstd, given);
+        if (r.k > kLargest) r.k = kLargest;                   // (zeros stay zeros, the rest saturates)
+        return r;
+    }
+    // rounding is monotonic: the largest |v| times rstd is the largest |v * rstd|.  127 / largest |v| takes rstd and the scale's rounding
+    // out of the codes.
+    const float top = a.int8 ? 127.0f : 448.0f, v = s.largest, y = v * r.rstd;
+    if (y == 0.0f) {
+        r.scale = 1.0f;
+        r.k = 0.0f;
+    } else if (y < kInfinity) {
+        r.scale = __fdiv_rn(y, top);
+        r.k = __fdiv_rn(top, v);
+        if (r.scale < kSmallest || r.k > kLargest) {
+            r.small = true;
+            r.scale = fmaxf(r.scale, kSmallest);
+            r.k = __frcp_rn(r.scale);
+        }
+    } else {
+        r.scale = r.k = nan;
     }
     return r;
 }
 
-constexpr int kRowThreads = 128;
-
-// A row by G threads, CH groups of eight elements each, read once and held in registers; statistics in fp32.  Bound by the bytes of
-// x, the residual, their sum and the codes.
-template <typename T, bool NORM, bool VEC, int G, int CH>
-__global__ void __launch_bounds__(G < kRowThreads ? kRowThreads : G) row_kernel(const RowArgs a) {
-    constexpr int BLOCK = G < kRowThreads ? kRowThreads : G, ROWS = BLOCK / G;
-    const int c0 = (threadIdx.x % G) * 8;
-    const float inv_n = 1.0f / static_cast<float>(a.cols);
+// A row by the threads of a block (or, WARP, of a warp), CH times eight elements each: read once and held in registers, everything
+// asked for before the first of it is used; statistics in fp32, four partial sums a thread.  Bound by the bytes of x, the
+// residual, their sum and the codes.
+constexpr int kWarpRowThreads = 128;
+template <typename T, bool NORM, bool VEC, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRowThreads : CH == 1 ? 1024 : 512) row_kernel(const RowArgs a) {
+    const int lane = threadIdx.x & 31;
+    const int c0 = (WARP ? 0 : (threadIdx.x >> 5) * 256) + (VEC ? 8 * lane : lane), c_step = WARP ? 256 : 8 * blockDim.x;
+    const auto column = [&](int j) { return c0 + c_step * j; };              // the first of the eight elements
+    constexpr int ROWS = WARP ? kWarpRowThreads / 32 : 1;                    // of the block at a time
     sl8::pdl_wait();
     sl8::pdl_release();
-    const float given_inv = a.row_scales ? 0.0f : __frcp_rn(a.scale ? sl8::ld_f32(a.scale) : 1.0f);
+    const float given = a.scale ? sl8::ld_f32(a.scale) : 1.0f;
+    extern __shared__ __align__(16) float row_gamma[];                       // the block's copy: read again for every row
+    if (NORM && a.gamma) {
+        constexpr int PER = VEC ? 4 : 1;
+        for (int c = PER * threadIdx.x; c < a.cols; c += PER * blockDim.x)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(sl8::smem_u32(row_gamma + c)), "l"(a.gamma + c), "n"(4 * PER) : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     int turn = 0;
-    for (long long r = static_cast<long long>(blockIdx.x) * ROWS + threadIdx.x / G; r < a.rows; r += static_cast<long long>(gridDim.x) * ROWS, turn++) {
+    for (long long r0 = static_cast<long long>(blockIdx.x) * ROWS; r0 < a.rows; r0 += static_cast<long long>(gridDim.x) * ROWS, turn++) {
+        const long long r = r0 + (WARP ? threadIdx.x >> 5 : 0);
+        const bool live = !WARP || r < a.rows;                               // this warp has a row
         const T* const x = static_cast<const T*>(a.x) + r * a.ld;
         float v[CH][8];
-        {
+        Stats s = {0.0f, 0.0f};
+        if constexpr (NORM) {
+            Eight<T> e[CH], f[CH];
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+                if (live && column(j) < a.cols) fetch<VEC>(e[j], x + column(j), a.cols - column(j));
+            if (live && a.residual) {
+                const T* const res = static_cast<const T*>(a.residual) + r * a.ld_res;
+#pragma unroll
+                for (int j = 0; j < CH; j++)
+                    if (column(j) < a.cols) fetch<VEC>(f[j], res + column(j), a.cols - column(j));
+            }
+            if (turn == 0 && a.gamma) {       // (with the first row's elements on their way)
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncthreads();
+            }
+            if (!live) continue;
+            float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < CH; j++)
+                if (column(j) < a.cols) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[j][i] = value(e[j], i);
+                    if (a.residual) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[j][i] += value(f[j], i);
+                        put_sum<VEC>(static_cast<T*>(a.sum) + r * a.ld_sum + column(j), v[j], a.cols - column(j));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) squares[i & 3] = fmaf(v[j][i], v[j][i], squares[i & 3]);
+                    if (a.gamma) times_gamma<VEC>(v[j], row_gamma + column(j), a.cols - column(j));
+                    s.largest = largest_of(s.largest, v[j]);
+                }
+            s.squares = (squares[0] + squares[1]) + (squares[2] + squares[3]);
+        } else {
+            if (!live) continue;
             Eight<T> e[CH];
 #pragma unroll
             for (int j = 0; j < CH; j++)
-                if (c0 + 8 * G * j < a.cols) fetch<VEC>(e[j], x + c0 + 8 * G * j, a.cols - (c0 + 8 * G * j));
-            if (NORM && a.residual) {
-                const T* const res = static_cast<const T*>(a.residual) + r * a.ld_res;
-                T* const sum = static_cast<T*>(a.sum) + r * a.ld_sum;
-                Eight<T> f[CH];
+                if (column(j) < a.cols) fetch<VEC>(e[j], x + column(j), a.cols - column(j));
 #pragma unroll
-                for (int j = 0; j < CH; j++)
-                    if (c0 + 8 * G * j < a.cols) fetch<VEC>(f[j], res + c0 + 8 * G * j, a.cols - (c0 + 8 * G * j));
-#pragma unroll
-                for (int j = 0; j < CH; j++)
-                    if (c0 + 8 * G * j < a.cols) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[j][i] = value(e[j], i) + value(f[j], i);
-                        put_sum<VEC>(sum + c0 + 8 * G * j, v[j], a.cols - (c0 + 8 * G * j));
-                    }
-            } else {
-#pragma unroll
-                for (int j = 0; j < CH; j++)
+            for (int j = 0; j < CH; j++)
+                if (column(j) < a.cols) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[j][i] = value(e[j], i);
-            }
-        }
-        Stats s = {0.0f, 0u};
-#pragma unroll
-        for (int j = 0; j < CH; j++)
-            if (c0 + 8 * G * j < a.cols) {
-                if constexpr (NORM) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s.squares = fmaf(v[j][i], v[j][i], s.squares);
-                    if (a.gamma) {
-                        Eight<float> g;
-                        fetch<VEC>(g, a.gamma + c0 + 8 * G * j, a.cols - (c0 + 8 * G * j));
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[j][i] *= value(g, i);
-                    }
+                    s.largest = largest_of(s.largest, v[j]);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; i++) s.largest = max(s.largest, magnitude(v[j][i]));
-            }
-        const Scaling k = scaling<NORM>(a, reduce<NORM, G>(s, turn), inv_n, given_inv);
+        }
+        const Scaling k = scaling<NORM>(a, WARP ? reduce_warp<NORM>(s) : reduce_block<NORM>(s, turn), given);
         uint8_t* const out = a.out + r * a.ld_out;
 #pragma unroll
         for (int j = 0; j < CH; j++)
-            if (c0 + 8 * G * j < a.cols) {
-                if constexpr (NORM) {
+            if (column(j) < a.cols) {
+                if (k.small) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[j][i] *= k.rstd;
                 }
-                put_codes<VEC>(out + c0 + 8 * G * j, v[j], k.inv, a.int8 != 0, a.cols - (c0 + 8 * G * j));
+                put_codes<VEC>(out + column(j), v[j], k.k, a.int8 != 0, a.cols - column(j));
             }
-        if (a.row_scales && threadIdx.x % G == 0) a.row_scales[r] = k.scale;
+        if (a.row_scales && (WARP ? lane : static_cast<int>(threadIdx.x)) == 0) a.row_scales[r] = k.scale;
+    }
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void shared_eight(Eight<T>& e, const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p + i * (16 / (int)sizeof(T)));
+        e.w[4 * i] = q.x; e.w[4 * i + 1] = q.y; e.w[4 * i + 2] = q.z; e.w[4 * i + 3] = q.w;
+    }
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void shared_values(float (&v)[8], const T* p, int left) {
+    if constexpr (VEC) {
+        Eight<T> e;
+        shared_eight(e, p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = value(e, i);
+    } else {
+        if (left > 224) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = static_cast<float>(p[32 * i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 32 * i < left ? static_cast<float>(p[32 * i]) : 0.0f;
+        }
+    }
+}
+
+constexpr int kSlots = 2;
+__host__ __device__ constexpr int gamma_bytes(bool given, int cols) { return given ? (cols + 255) / 256 * 1024 : 0; }
+template <typename T, bool NORM, bool VEC, int CH, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRowThreads : 512) row_stream_kernel(const RowArgs a, int span) {
+    constexpr int GROUPS = WARP ? kWarpRowThreads / 32 : 1;
+    extern __shared__ __align__(128) uint8_t stream_smem[];
+    __shared__ __align__(8) uint64_t bars[GROUPS * kSlots];
+    __shared__ volatile uint32_t abort_flag;
+    const int lane = threadIdx.x & 31, group = WARP ? threadIdx.x >> 5 : 0;
+    const bool lead = WARP ? lane == 0 : threadIdx.x == 0;
+    const int c0 = (WARP ? 0 : (threadIdx.x >> 5) * 256) + (VEC ? 8 * lane : lane), c_step = WARP ? 256 : 8 * blockDim.x;
+    const auto column = [&](int j) { return c0 + c_step * j; };
+    const bool gamma = NORM && a.gamma, residual = NORM && a.residual;
+    float* const g = reinterpret_cast<float*>(stream_smem);
+    const int slot_bytes = residual ? 2 * span : span;
+    uint8_t* const slots = stream_smem + gamma_bytes(gamma, a.cols) + group * kSlots * slot_bytes;
+    const uint32_t bar0 = sl8::smem_u32(bars + group * kSlots);
+    sl8::WaitCtx wc;
+    wc.abort_flag = &abort_flag;
+    wc.peer_abort = 0u;
+    wc.status = a.status;
+    wc.budget_ns = static_cast<unsigned long long>(a.wait_budget_us) * 1000ull;
+    wc.tile = 0;
+    if (lead) {
+        for (int s = 0; s < kSlots; s++) sl8::mbar_init(bar0 + 8 * s, 1);
+        sl8::fence_mbar_init();
+        if (group == 0) abort_flag = 0u;
+    }
+    sl8::pdl_wait();
+    sl8::pdl_release();
+    const float given = a.scale ? sl8::ld_f32(a.scale) : 1.0f;
+    const long long stride = static_cast<long long>(gridDim.x) * GROUPS;
+    // Bytes of a row from the 16-byte boundary at or below its start to the one at or above its end.  What sticks out belongs to the rows
+    // beside it (a row has at least 16 bytes); of the first and the last row it may not belong to the caller, so these are read element by element.
+    const auto apart = [&](long long r) { return !VEC && (r == 0 || r == a.rows - 1); };
+    const auto issue = [&](int s, long long r) {
+        if (r >= a.rows || apart(r) || !lead) return;
+        const uint32_t dst = sl8::smem_u32(slots + s * slot_bytes), bar = bar0 + 8 * s;
+        const auto one = [&](const void* p, long long ld, uint32_t to, bool copy) {
+            const uintptr_t from = reinterpret_cast<uintptr_t>(p) + r * ld * sizeof(T), start = from & ~uintptr_t{15};
+            const uint32_t bytes = static_cast<uint32_t>((from + a.cols * sizeof(T) + 15) / 16 * 16 - start);
+            if (copy) bulk_load(to, reinterpret_cast<const void*>(start), bytes, bar);
+            return bytes;
+        };
+        const uint32_t total = one(a.x, a.ld, dst, false) + (residual ? one(a.residual, a.ld_res, dst + span, false) : 0u);
+        if (!VEC) sl8::fence_proxy_async_smem();       // (rows that are read element by element are written to their slot)
+        sl8::mbar_arrive_expect_tx(bar, total);
+        if (!(a.drop && r == 1)) one(a.x, a.ld, dst, true);
+        if (residual) one(a.residual, a.ld_res, dst + span, true);
+    };
+    long long r = blockIdx.x * static_cast<long long>(GROUPS) + group;
+    for (int s = 0; s < kSlots; s++) issue(s, r + s * stride);
+    if (gamma) {
+        constexpr int PER = VEC ? 4 : 1;
+        for (int c = PER * threadIdx.x; c < a.cols; c += PER * blockDim.x) {
+            // VEC: the two halves of a lane's eight 128 elements apart, so that the lanes' reads meet no bank twice
+            const int to = VEC ? (c & ~255) + ((c & 4) ? 128 : 0) + (c & 255) / 8 * 4 : c;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(sl8::smem_u32(g + to)), "l"(a.gamma + c), "n"(4 * PER) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    __syncthreads();
+    uint32_t phases = 0u;
+    for (int turn = 0, s = 0; r < a.rows; r += stride, turn++, s = s + 1 == kSlots ? 0 : s + 1) {
+        uint8_t* const slot = slots + s * slot_bytes;
+        const auto place = [&](const void* p, long long ld, uint8_t* at) {        // where the row's elements lie in the slot
+            return reinterpret_cast<T*>(at + (VEC ? 0 : (reinterpret_cast<uintptr_t>(p) + r * ld * sizeof(T)) & 15));
+        };
+        T* const x = place(a.x, a.ld, slot);
+        T* const res = place(a.residual, a.ld_res, slot + span);
+        bool ok = true;
+        if (apart(r)) {
+            const int first = WARP ? lane : threadIdx.x, step = WARP ? 32 : blockDim.x;
+            for (int c = first; c < a.cols; c += step) {
+                x[c] = static_cast<const T*>(a.x)[r * a.ld + c];
+                if (residual) res[c] = static_cast<const T*>(a.residual)[r * a.ld_res + c];
+            }
+            if (WARP) __syncwarp();
+            else __syncthreads();
+        } else {
+            wc.tile = static_cast<uint32_t>(r);
+            ok = sl8::wait_bar<true>(bar0 + 8 * s, (phases >> s) & 1u, wc, sl8::ST_ROW_WAIT, s);
+            phases ^= 1u << s;
+        }
+        if (WARP && !__all_sync(0xffffffffu, ok)) break;
+        float v[CH][8];
+        Stats st = {0.0f, 0.0f};
+        float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+            if (column(j) < a.cols) {
+                const int left = a.cols - column(j);
+                shared_values<VEC>(v[j], x + column(j), left);
+                if constexpr (NORM) {
+                    if (residual) {
+                        float f[8];
+                        shared_values<VEC>(f, res + column(j), left);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[j][i] += f[i];
+                        put_sum<VEC>(static_cast<T*>(a.sum) + r * a.ld_sum + column(j), v[j], left);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) squares[i & 3] = fmaf(v[j][i], v[j][i], squares[i & 3]);
+                    if (gamma) {
+                        if constexpr (VEC) {
+                            const float* const at = g + (column(j) & ~255) + 4 * lane;
+                            const float4 lo = *reinterpret_cast<const float4*>(at), hi = *reinterpret_cast<const float4*>(at + 128);
+                            v[j][0] *= lo.x; v[j][1] *= lo.y; v[j][2] *= lo.z; v[j][3] *= lo.w;
+                            v[j][4] *= hi.x; v[j][5] *= hi.y; v[j][6] *= hi.z; v[j][7] *= hi.w;
+                        } else {
+                            times_gamma<VEC>(v[j], g + column(j), left);
+                        }
+                    }
+                }
+                st.largest = largest_of(st.largest, v[j]);
+            }
+        st.squares = (squares[0] + squares[1]) + (squares[2] + squares[3]);
+        st = WARP ? reduce_warp<NORM>(st) : reduce_block<NORM>(st, turn);
+        if (WARP) __syncwarp();
+        else if (abort_flag) break;              // (set ahead of the barrier by whoever gave up: seen by all)
+        issue(s, r + kSlots * stride);
+        const Scaling k = scaling<NORM>(a, st, given);
+        uint8_t* const out = a.out + r * a.ld_out;
+#pragma unroll
+        for (int j = 0; j < CH; j++)
+            if (column(j) < a.cols) {
+                if (k.small) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[j][i] *= k.rstd;
+                }
+                put_codes<VEC>(out + column(j), v[j], k.k, a.int8 != 0, a.cols - column(j));
+            }
+        if (a.row_scales && lead) a.row_scales[r] = k.scale;
+    }
+    if (abort_flag) {          // copies in flight land before their memory is released
+        const unsigned long long t0 = sl8::globaltimer_ns();
+        while (sl8::globaltimer_ns() - t0 < 200000ull) {
+        }
     }
 }
 
 // Rows too long for the registers of a block: read twice, statistics first.  The sum is written the second time only, because it may
-// lie where the first reading still has to find x or the residual.
+// lie where the second reading still has to find x or the residual.
 constexpr int kLongThreads = 512;
 template <typename T, bool NORM, bool VEC>
 __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const RowArgs a) {
-    const float inv_n = 1.0f / static_cast<float>(a.cols);
+    const int first = VEC ? 8 * threadIdx.x : (threadIdx.x >> 5) * 256 + (threadIdx.x & 31);
     sl8::pdl_wait();
     sl8::pdl_release();
-    const float given_inv = a.row_scales ? 0.0f : __frcp_rn(a.scale ? sl8::ld_f32(a.scale) : 1.0f);
+    const float given = a.scale ? sl8::ld_f32(a.scale) : 1.0f;
     int turn = 0;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x, turn++) {
         const T* const x = static_cast<const T*>(a.x) + r * a.ld;
-        const T* const res = NORM && a.residual ? static_cast<const T*>(a.residual) + r * a.ld_res : nullptr;
-        T* const sum = static_cast<T*>(a.sum) + r * a.ld_sum;
+        // h of the group at column c
         const auto load = [&](int c, float (&v)[8], bool write) {
-            Eight<T> e;
+            Eight<T> e, f;
             fetch<VEC>(e, x + c, a.cols - c);
+            if (NORM && a.residual) fetch<VEC>(f, static_cast<const T*>(a.residual) + r * a.ld_res + c, a.cols - c);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = value(e, i);
-            if (res) {
-                fetch<VEC>(e, res + c, a.cols - c);
+            if (NORM && a.residual) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] += value(e, i);
-                if (write) put_sum<VEC>(sum + c, v, a.cols - c);
+                for (int i = 0; i < 8; i++) v[i] += value(f, i);
+                if (write) put_sum<VEC>(static_cast<T*>(a.sum) + r * a.ld_sum + c, v, a.cols - c);
             }
         };
-        const auto times_gamma = [&](int c, float (&v)[8]) {
+        const auto scaled = [&](int c, float (&v)[8]) {
             if (NORM && a.gamma) {
                 Eight<float> g;
                 fetch<VEC>(g, a.gamma + c, a.cols - c);
@@ -270,49 +503,107 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const RowArgs a)
                 for (int i = 0; i < 8; i++) v[i] *= value(g, i);
             }
         };
-        Stats s = {0.0f, 0u};
-        for (int c = threadIdx.x * 8; c < a.cols; c += 8 * kLongThreads) {
+        Stats s = {0.0f, 0.0f};
+        float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = first; c < a.cols; c += 8 * kLongThreads) {
             float v[8];
             load(c, v, false);
             if constexpr (NORM) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) s.squares = fmaf(v[i], v[i], s.squares);
-                times_gamma(c, v);
+                for (int i = 0; i < 8; i++) squares[i & 3] = fmaf(v[i], v[i], squares[i & 3]);
+                scaled(c, v);
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) s.largest = max(s.largest, magnitude(v[i]));
+            s.largest = largest_of(s.largest, v);
         }
-        const Scaling k = scaling<NORM>(a, reduce<NORM, kLongThreads>(s, turn), inv_n, given_inv);
-        for (int c = threadIdx.x * 8; c < a.cols; c += 8 * kLongThreads) {
+        s.squares = (squares[0] + squares[1]) + (squares[2] + squares[3]);
+        const Scaling k = scaling<NORM>(a, reduce_block<NORM>(s, turn), given);
+        for (int c = first; c < a.cols; c += 8 * kLongThreads) {
             float v[8];
             load(c, v, true);
-            if constexpr (NORM) {
-                times_gamma(c, v);
+            scaled(c, v);
+            if (k.small) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[i] *= k.rstd;
             }
-            put_codes<VEC>(a.out + r * a.ld_out + c, v, k.inv, a.int8 != 0, a.cols - c);
+            put_codes<VEC>(a.out + r * a.ld_out + c, v, k.k, a.int8 != 0, a.cols - c);
         }
         if (a.row_scales && threadIdx.x == 0) a.row_scales[r] = k.scale;
     }
 }
 
+// ---- which kernel, on how many blocks
+constexpr size_t kRingBytes = 227 * 1024 - 1024;       // shared memory of a block, less what the kernel declares itself
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, size_t bytes) {
+    return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+}
+
+template <typename T, bool NORM, bool VEC>
+cudaError_t launch_long(int sm_count, cudaStream_t s, const RowArgs& a) {
+    const long long cap = static_cast<long long>(sm_count) * 8;
+    return sl8_launch_chained(long_row_kernel<T, NORM, VEC>, static_cast<unsigned>(a.rows < cap ? a.rows : cap), kLongThreads, 0, s, a);
+}
+
+template <typename T, bool NORM, bool VEC, int CH, bool WARP>
+cudaError_t direct(int sm_count, cudaStream_t s, const RowArgs& a) {
+    const auto kernel = row_kernel<T, NORM, VEC, CH, WARP>;
+    const size_t bytes = NORM && a.gamma ? sizeof(float) * a.cols : 0;
+    const cudaError_t e = allow_shared(kernel, bytes);
+    if (e != cudaSuccess) return e;
+    constexpr int ROWS = WARP ? kWarpRowThreads / 32 : 1;
+    const int threads = WARP ? kWarpRowThreads : ((a.cols + 7) / 8 + CH * 32 - 1) / (CH * 32) * 32;
+    const long long want = (a.rows + ROWS - 1) / ROWS, cap = static_cast<long long>(sm_count) * (WARP ? 16 : 8);
+    return sl8_launch_chained(kernel, static_cast<unsigned>(want < cap ? want : cap), threads, bytes, s, a);
+}
+
+template <typename T, bool NORM, bool VEC, int CH, bool WARP>
+cudaError_t stream_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
+    const auto kernel = row_stream_kernel<T, NORM, VEC, CH, WARP>;
+    static const int regs = [&] {                       // of the kernel, looked up once
+        cudaFuncAttributes fa = {};
+        return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess && fa.numRegs > 0 ? fa.numRegs : 64;
+    }();
+    constexpr int GROUPS = WARP ? kWarpRowThreads / 32 : 1;
+    const int span = (a.cols * static_cast<int>(sizeof(T)) + 16 + 127) / 128 * 128;
+    const size_t bytes = gamma_bytes(NORM && a.gamma, a.cols) + static_cast<size_t>(GROUPS) * kSlots * span * (a.residual ? 2 : 1);
+    if (bytes > kRingBytes) return launch_long<T, NORM, VEC>(sm_count, s, a);
+    const cudaError_t e = allow_shared(kernel, bytes);
+    if (e != cudaSuccess) return e;
+    const int threads = WARP ? kWarpRowThreads : ((a.cols + 7) / 8 + CH * 32 - 1) / (CH * 32) * 32;
+    // Blocks that are resident at once, and from some rows per block on several times as many: the SMs do not get through their rows
+    // equally fast.  Each block brings gamma once, so that one with gamma takes more rows.
+    const int by_regs = 65536 / ((regs + 7) / 8 * 8 * threads), by_bytes = static_cast<int>(228 * 1024 / (bytes + 2048)), by_warps = 2048 / threads;
+    int resident = by_regs < by_bytes ? by_regs : by_bytes;
+    if (by_warps < resident) resident = by_warps;
+    if (resident < 1) resident = 1;
+    const long long want = (a.rows + GROUPS - 1) / GROUPS, once = static_cast<long long>(sm_count) * resident;
+    long long waves = want / once / (WARP ? 4 : NORM && a.gamma ? 16 : 8);
+    waves = want <= 2 * once ? 2 : waves < 1 ? 1 : waves > 4 ? 4 : waves;
+    return sl8_launch_chained(kernel, static_cast<unsigned>(want < once * waves ? want : once * waves), threads, bytes, s, a, span);
+}
+
+// Few rows: a block each, one trip to memory; from then on a warp each while rows are short, as long as there is hardly a second row
+// for a warp; then, and where rows start on odd addresses, the ring in shared memory.
 template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
-    const auto go = [&](auto kernel, int g, int threads, int per_sm) {
-        const long long want = (a.rows + threads / g - 1) / (threads / g), cap = static_cast<long long>(sm_count) * per_sm;
-        return sl8_launch_chained(kernel, static_cast<unsigned>(want < cap ? want : cap), threads, 0, s, a);
-    };
-#define SL8_ROWS(G, CH, PER_SM) go(row_kernel<T, NORM, VEC, G, CH>, G, G < kRowThreads ? kRowThreads : G, PER_SM)
-    if (a.cols <= 256) return SL8_ROWS(32, 1, 32);
-    if (a.cols <= 768) return SL8_ROWS(32, 3, 32);
-    if (a.cols <= 1280) return SL8_ROWS(32, 5, 32);
-    if (a.cols <= 2048) return SL8_ROWS(128, 2, 32);
-    if (a.cols <= 4096) return SL8_ROWS(128, 4, 32);
-    if (a.cols <= 8192) return SL8_ROWS(256, 4, 16);
-    if (a.cols <= 16384) return SL8_ROWS(512, 4, 8);
-#undef SL8_ROWS
-    return go(long_row_kernel<T, NORM, VEC>, kLongThreads, kLongThreads, 8);
+    const bool few = a.rows <= 10ll * sm_count;
+    if (few || a.cols * sizeof(T) < 16) {
+        if (a.cols <= 2048) return direct<T, NORM, VEC, 1, false>(sm_count, s, a);
+        if (a.cols <= 12288) return direct<T, NORM, VEC, 3, false>(sm_count, s, a);
+    }
+    if constexpr (VEC) {
+        if (a.rows <= 40ll * sm_count && a.cols <= 1280)
+            return a.cols <= 256 ? direct<T, NORM, true, 1, true>(sm_count, s, a) : a.cols <= 768 ? direct<T, NORM, true, 3, true>(sm_count, s, a) : direct<T, NORM, true, 5, true>(sm_count, s, a);
+        if (a.cols > 768 && a.cols <= 1280) return stream_rows<T, NORM, true, 5, true>(sm_count, s, a);
+    }
+    if (a.cols <= 256) return stream_rows<T, NORM, VEC, 1, true>(sm_count, s, a);
+    if (a.cols <= 512) return stream_rows<T, NORM, VEC, 2, true>(sm_count, s, a);
+    if (a.cols <= 768) return stream_rows<T, NORM, VEC, 3, true>(sm_count, s, a);
+    if constexpr (!VEC)
+        if (a.cols <= 2048) return stream_rows<T, NORM, false, 2, false>(sm_count, s, a);
+    if (a.cols <= 12288) return stream_rows<T, NORM, VEC, 3, false>(sm_count, s, a);
+    if (a.cols <= 16384) return stream_rows<T, NORM, VEC, 4, false>(sm_count, s, a);
+    return launch_long<T, NORM, VEC>(sm_count, s, a);
 }
 
 template <typename T, bool NORM>
@@ -346,6 +637,7 @@ SL8_API int sl8_quantize_rows(sl8_handle_t h, const void* x, int dtype, int64_t 
     a.x = x; a.ld = ld;
     a.out = static_cast<uint8_t*>(out); a.ld_out = ld_out;
     a.row_scales = row_scales; a.rows = rows; a.cols = cols; a.int8 = code_type == SL8_CODE_INT8;
+    a.status = h->d_status; a.wait_budget_us = h->wait_budget_us; a.drop = h->test_drop_b;
     return dtype == SL8_DT_F32 ? run_rows<float, false>(h, a, stream, "quantize_rows kernel launch") : run_rows<bf16, false>(h, a, stream, "quantize_rows kernel launch");
 }
 
@@ -370,5 +662,6 @@ SL8_API int sl8_rmsnorm_quantize(sl8_handle_t h, const void* x, int dtype, int64
     a.gamma = gamma; a.eps = eps; a.scale = scale;
     a.out = static_cast<uint8_t*>(out); a.ld_out = ld_out;
     a.row_scales = row_scales; a.rows = rows; a.cols = cols; a.int8 = code_type == SL8_CODE_INT8;
+    a.status = h->d_status; a.wait_budget_us = h->wait_budget_us; a.drop = h->test_drop_b;
     return dtype == SL8_DT_F32 ? run_rows<float, true>(h, a, stream, "rmsnorm kernel launch") : run_rows<bf16, true>(h, a, stream, "rmsnorm kernel launch");
 }

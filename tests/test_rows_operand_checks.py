@@ -151,7 +151,7 @@ def test_null_handles():
 def test_the_predicted_codes_are_half_a_step_off_at_most(oracle):
     """The prediction that test_rows.py holds the kernels to, bit for bit, against the definition in 64 bits."""
     from tests.test_prep import nearest_e4m3
-    from tests.test_rows import row_scales_of
+    from tests.test_rows import row_factors_of, row_scales_of
     rng = np.random.default_rng(0)
     y = (rng.standard_normal((200, 333)) * np.exp(rng.standard_normal((200, 1)) * 8)).astype(np.float32)
     y[3] = 0
@@ -160,13 +160,13 @@ def test_the_predicted_codes_are_half_a_step_off_at_most(oracle):
     for top, half in ((127.0, lambda v, s: np.broadcast_to(s / 2, v.shape)), (448.0, lambda v, s: np.maximum(np.abs(v) / 16, s * 2.0 ** -10))):
         scale = row_scales_of(y, top)
         assert scale[3] == 1.0 and scale[4] == np.float32(2.0 ** -126)
-        inv = (np.float32(1) / scale).astype(np.float32)[:, None]
-        assert np.isfinite(inv).all()
+        k = row_factors_of(y, top)[:, None]
+        assert np.isfinite(k).all()
         if top == 127.0:
-            v = np.rint(y.astype(np.float64) * inv)
+            v = np.rint(y.astype(np.float64) * k)
             assert np.abs(v).max() == 127
         else:
-            v = oracle.e4m3_lut().astype(np.float64)[nearest_e4m3(oracle, (y * inv).astype(np.float32))]
+            v = oracle.e4m3_lut().astype(np.float64)[nearest_e4m3(oracle, (y * k).astype(np.float32))]
             assert np.abs(v).max() == 448
         s = scale.astype(np.float64)[:, None]
         assert (np.abs(v * s - y) <= half(y, s) + np.abs(y) * 2.0 ** -22).all()
