@@ -281,7 +281,7 @@ int run_few(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
                    (unsigned long long)q.lda, 128, (unsigned)sl8::few_tile_rows(p.M), CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != SL8_OK) return rc;
     h->last_grid = 0;        // these kernels write no trace records
-    const cudaError_t e = sl8::few_launch(q.op == kOpInt8, sl8::few_split(h->sm_count, q.N, p.k_blocks), map_b, map_a, p, stream);
+    const cudaError_t e = sl8::few_launch(q.op == kOpInt8, h->sm_count, map_b, map_a, p, stream);
     return e == cudaSuccess ? SL8_OK : fail_cuda(h, e, "kernel launch");
 }
 
@@ -291,7 +291,7 @@ int run(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
     std::lock_guard<std::mutex> lock(h->mu);
     DeviceGuard guard(h->device);
     if (!guard.ok) return fail(h, SL8_ERR_CUDA, "cudaSetDevice failed");
-    if (sl8::op_scaled(q.op) && h->forced_variant < 0 && q.M <= sl8::kFewRowsMax) return run_few(h, q, stream);
+    if (sl8::op_scaled(q.op) && h->forced_variant < 0 && sl8::few_rows(q.M, q.K)) return run_few(h, q, stream);
 
     int vid = h->forced_variant >= 0 ? h->forced_variant : pick_variant(h, q.op, q.out_dtype, q.M, q.N, q.K, q.flags);
     const VariantEntry* v = variant(vid);

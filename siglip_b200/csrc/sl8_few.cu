@@ -14,21 +14,29 @@ namespace {
 template <int ROWS>
 struct FewTraits {
     static constexpr int W_BYTES = 128 * 128, STAGE_BYTES = W_BYTES + ROWS * 128;
-    static constexpr int STAGES = ROWS == 16 ? 6 : ROWS == 32 ? 5 : 4;      // about 100 KiB: two CTAs fit an SM
-    static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + 256;
+    static constexpr int SUM_BYTES = (ROWS < 4 * kFewSplitMax ? 4 * kFewSplitMax : ROWS) * 128 * 4;   // partial sums of the rows this CTA finishes
+    static constexpr int VEC_FLOATS = 2 * 128 + ROWS;                       // column scales, bias, row scales
+    // The ring: deep where every CTA has an SM of its own, else such that two CTAs fit one.
+    static constexpr int DEEP = ROWS == 64 ? 7 : 8, HALF = ROWS == 16 ? 5 : ROWS == 32 ? 4 : 3;
+    static constexpr int smem_bytes(int stages) { return 1024 + stages * STAGE_BYTES + SUM_BYTES + 4 * VEC_FLOATS + 256; }
+    static_assert(smem_bytes(DEEP) <= 232448 && 2 * (smem_bytes(HALF) + 1024) <= 228 * 1024, "one and two CTAs per SM");
+    static_assert(2 * DEEP + 1 <= 32 && 16 * DEEP + 16 <= 256, "a barrier per lane; room for them");
     static constexpr int TMEM_COLS = ROWS < 32 ? 32 : ROWS;
     static_assert(STAGE_BYTES % 1024 == 0, "every operand tile starts on a swizzle-atom boundary");
-    static_assert(ROWS * 128 * 4 <= STAGES * STAGE_BYTES, "partial sums fit where the operands were");
 };
 
 constexpr int kFewThreads = 128;
 
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_16(uint32_t addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
-__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
 
 template <bool I8, int ROWS>
 __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, const FewParams p) {
@@ -36,9 +44,11 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     extern __shared__ uint8_t few_smem[];
     const uint32_t raw = smem_u32(few_smem);
     const uint32_t base = (raw + 1023u) & ~1023u;
-    uint8_t* const bar_ptr = few_smem + (base - raw) + T::STAGES * T::STAGE_BYTES;
-    const uint32_t full0 = base + T::STAGES * T::STAGE_BYTES, empty0 = full0 + 8 * T::STAGES, done = empty0 + 8 * T::STAGES;
-    volatile uint32_t* const tmem_ptr = reinterpret_cast<volatile uint32_t*>(bar_ptr + 16 * T::STAGES + 8);
+    const uint32_t sums = base + p.stages * T::STAGE_BYTES;                            // [rank][128][rows of this CTA]
+    float* const vec = reinterpret_cast<float*>(few_smem + (sums - raw) + T::SUM_BYTES);  // column scales, bias, row scales
+    uint8_t* const bar_ptr = reinterpret_cast<uint8_t*>(vec + T::VEC_FLOATS);
+    const uint32_t full0 = sums + T::SUM_BYTES + 4 * T::VEC_FLOATS, empty0 = full0 + 8 * p.stages, done = empty0 + 8 * p.stages;
+    volatile uint32_t* const tmem_ptr = reinterpret_cast<volatile uint32_t*>(bar_ptr + 16 * p.stages + 8);
     volatile uint32_t* const abort_flag = tmem_ptr + 1;
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -56,7 +66,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     wc.tile = blockIdx.x / split;
 
     if (warp == 0) {
-        if (lane < 2 * T::STAGES + 1) {
+        if (lane < 2 * p.stages + 1) {
             mbar_init(full0 + 8 * lane, 1);
             fence_mbar_init();
         }
@@ -69,7 +79,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
             prefetch_tensormap(&map_b);
             prefetch_tensormap(&map_a);
             // (weights on their way into L2 while the kernel ahead finishes: a hint, like that of the other GEMMs)
-            for (int kb = kb_begin; kb < kb_end && kb < kb_begin + T::STAGES; kb++) tma_prefetch_l2_2d(&map_b, kb * 128, n0);
+            for (int kb = kb_begin; kb < kb_end && kb < kb_begin + p.stages; kb++) tma_prefetch_l2_2d(&map_b, kb * 128, n0);
         }
     }
     __syncwarp();
@@ -77,15 +87,9 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+    if (split > 1) cluster_arrive();         // (every CTA of the cluster runs before one writes to another's shared memory)
     pdl_wait();
     pdl_release();       // (behind the allocation of tensor memory, on which no later kernel may be ahead of this one)
-
-    const int n = n0 + static_cast<int>(threadIdx.x);       // this thread's output channel: TMEM lane threadIdx.x
-    float col_scale = 0.0f, bias = 0.0f;
-    if (n < p.N) {
-        col_scale = ld_f32(p.col_scales + n);
-        if (p.bias) bias = (p.flags & FLAG_BIAS_F32) ? ld_f32(static_cast<const float*>(p.bias) + n) : ld_bf16(static_cast<const __nv_bfloat16*>(p.bias) + n);
-    }
 
     if (warp == 0) {
         int stage = 0;
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
                 tma_load_2d(dst, &map_b, kb * 128, n0, bar);
             }
             __syncwarp();
-            if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
+            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         }
     } else if (warp == 1) {
         const uint32_t idesc = I8 ? make_idesc_i8_s32(128, ROWS) : make_idesc_e4m3_f32(128, ROWS);
@@ -126,68 +130,94 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
                 if (kb == kb_end - 1) mma_commit(done);
             }
             __syncwarp();
-            if (++stage == T::STAGES) { stage = 0; phase ^= 1u; }
+            if (++stage == p.stages) { stage = 0; phase ^= 1u; }
         }
     }
-    __syncwarp();
-    const bool ok = __all_sync(0xffffffffu, wait_bar(done, 0, wc, ST_EPI_TMEM_FULL_WAIT, 0)) != 0;
+    if (warp >= 2) {
+        // while the operands come: what the sums are multiplied with
+        for (int i = threadIdx.x - 64; i < 128; i += 64) {
+            float col_scale = 0.0f, bias = 0.0f;
+            if (n0 + i < p.N) {
+                col_scale = ld_f32(p.col_scales + n0 + i);
+                if (p.bias) bias = (p.flags & FLAG_BIAS_F32) ? ld_f32(static_cast<const float*>(p.bias) + n0 + i) : ld_bf16(static_cast<const __nv_bfloat16*>(p.bias) + n0 + i);
+            }
+            vec[i] = col_scale;
+            vec[128 + i] = bias;
+        }
+        for (int i = threadIdx.x - 64; i < p.M; i += 64) vec[256 + i] = ld_f32(p.row_scales + i);
+    }
+    __syncthreads();
+    const bool ok = __all_sync(0xffffffffu, wait_bar<true>(done, 0, wc, ST_EPI_TMEM_FULL_WAIT, 0)) != 0;
     tc_fence_after();
 
-    const auto sum_of = [](uint32_t a, uint32_t b) { return I8 ? a + b : __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); };
-    const auto finish = [&](int m, uint32_t sum) {
-        const float acc = I8 ? __int2float_rn(static_cast<int>(sum)) : __uint_as_float(sum);
-        float y = fmaf(acc * ld_f32(p.row_scales + m), col_scale, bias);
+    const int n = n0 + static_cast<int>(threadIdx.x);       // this thread's output channel: TMEM lane threadIdx.x
+    const float col_scale = vec[threadIdx.x], bias = vec[128 + threadIdx.x];
+    const auto sum_of = [](float a, float b) { return I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b; };
+    const auto number = [](float sum) { return I8 ? __int2float_rn(__float_as_int(sum)) : sum; };
+    // rows m .. m + 3 of this channel, as far as there are so many
+    const auto finish4 = [&](int m, float s0, float s1, float s2, float s3) {
+        const float4 row = *reinterpret_cast<const float4*>(vec + 256 + m);
+        float y[4] = {fmaf(number(s0) * row.x, col_scale, bias), fmaf(number(s1) * row.y, col_scale, bias),
+                      fmaf(number(s2) * row.z, col_scale, bias), fmaf(number(s3) * row.w, col_scale, bias)};
         if (!(p.flags & FLAG_NO_ACTIVATION)) {
-            float unused;
-            unpack_f32x2(gelu_tanh_x2(pack_f32x2(y, 0.0f)), y, unused);
+            unpack_f32x2(gelu_tanh_x2(pack_f32x2(y[0], y[1])), y[0], y[1]);
+            unpack_f32x2(gelu_tanh_x2(pack_f32x2(y[2], y[3])), y[2], y[3]);
         }
-        if (n < p.N) static_cast<__nv_bfloat16*>(p.D)[m * p.ldd + n] = __float2bfloat16_rn(y);
+        if (n < p.N) {
+            __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.D) + m * p.ldd + n;
+#pragma unroll
+            for (int i = 0; i < 4; i++, d += p.ldd)
+                if (m + i < p.M) *d = __float2bfloat16_rn(y[i]);
+        }
     };
     const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    constexpr int CHUNK = 16;
     if (split == 1) {
         if (ok) {
 #pragma unroll 1
-            for (int c = 0; c < p.M; c += 32) {
-                float v[32];
-                tmem_ld_32x32(t_row + c, v);       // (of 16 rows: with 16 columns that nothing wrote and nothing uses)
+            for (int c = 0; c < p.M; c += CHUNK) {
+                float v[CHUNK];
+                tmem_ld_32x16(t_row + c, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (c + i < p.M) finish(c + i, __float_as_uint(v[i]));
+                for (int i = 0; i < CHUNK; i += 4)
+                    if (c + i < p.M) finish4(c + i, v[i], v[i + 1], v[i + 2], v[i + 3]);
             }
         }
     } else {
-        // Sums of row m, column n0 + i: at base + (m * 128 + i) * 4, where the operands were (every copy has landed and been read).
-        const uint32_t mine = base + 4 * threadIdx.x;
+        // Each rank of the cluster finishes `share` rows, a multiple of four: it gets their sums from every rank.
+        const int share = p.share, own = static_cast<int>(rank) * share;
+        cluster_wait();
         if (ok) {
+            int owner = 0, at = 0;
 #pragma unroll 1
-            for (int c = 0; c < p.M; c += 32) {
-                float v[32];
-                tmem_ld_32x32(t_row + c, v);
+            for (int c = 0; c < p.M; c += CHUNK) {
+                float v[CHUNK];
+                tmem_ld_32x16(t_row + c, v);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (c + i < p.M) sts32(mine + (c + i) * 512, __float_as_uint(v[i]));
+                for (int i = 0; i < CHUNK; i += 4)
+                    if (c + i < p.M) {
+                        st_cluster_16(map_to_cta(sums + ((rank * 128 + threadIdx.x) * share + at) * 4, owner), v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        at += 4;
+                        if (at == share) at = 0, owner++;
+                    }
             }
         }
         __syncwarp();
         cluster_arrive();
-        cluster_wait();
-        const int m_end = static_cast<int>(p.M * (rank + 1) / split);
-        for (int m = static_cast<int>(p.M * rank / split); m < m_end; m++) {
-            uint32_t part[kFewSplitMax];
-#pragma unroll
-            for (int q = 0; q < kFewSplitMax; q++)
-                if (q < static_cast<int>(split)) part[q] = ld_cluster(map_to_cta(mine + m * 512, q));
-            uint32_t sum = part[0];
-#pragma unroll
-            for (int q = 1; q < kFewSplitMax; q++)
-                if (q < static_cast<int>(split)) sum = sum_of(sum, part[q]);
-            finish(m, sum);
+        if (own < p.M) {               // (a CTA that finishes no row is written to by none)
+            cluster_wait();
+            const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + threadIdx.x * share;
+            for (int i = 0; i < share && own + i < p.M; i += 4) {
+                float4 s = *reinterpret_cast<const float4*>(mine + i);
+                for (uint32_t q = 1; q < split; q++) {
+                    const float4 o = *reinterpret_cast<const float4*>(mine + q * 128 * share + i);
+                    s = make_float4(sum_of(s.x, o.x), sum_of(s.y, o.y), sum_of(s.z, o.z), sum_of(s.w, o.w));
+                }
+                finish4(own + i, s.x, s.y, s.z, s.w);
+            }
         }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();        // its sums have been read
     }
 
     tc_fence_before();
@@ -204,16 +234,29 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     }
 }
 
+// CTAs that share the K of one block of 128 columns: as many as give each SM one, with at least one and a half k-blocks for each.
+int few_split(int sm_count, int N, int k_blocks) {
+    const int blocks = (N + 127) / 128;
+    int split = 1;
+    while (split < kFewSplitMax && blocks * split * 2 <= sm_count && split * 3 <= k_blocks) split *= 2;
+    return split;
+}
+
 template <bool I8, int ROWS>
-cudaError_t launch(int split, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream) {
+cudaError_t launch(int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, FewParams p, cudaStream_t stream) {
+    const int split = few_split(sm_count, p.N, p.k_blocks);
     using T = FewTraits<ROWS>;
     const auto kernel = few_rows_kernel<I8, ROWS>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_BYTES);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::smem_bytes(T::DEEP));
     if (e != cudaSuccess) return e;
+    const int ctas = (p.N + 127) / 128 * split, most = (p.k_blocks + split - 1) / split;
+    p.stages = ctas <= sm_count ? T::DEEP : T::HALF;
+    if (p.stages > most) p.stages = most;            // (a short ring leaves room for the next kernel's CTAs)
+    p.share = (p.M + 4 * split - 1) / (4 * split) * 4;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((p.N + 127) / 128 * split), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
     cfg.blockDim = dim3(kFewThreads, 1, 1);
-    cfg.dynamicSmemBytes = T::SMEM_BYTES;
+    cfg.dynamicSmemBytes = static_cast<size_t>(T::smem_bytes(p.stages));
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -231,17 +274,11 @@ cudaError_t launch(int split, const CUtensorMap& map_b, const CUtensorMap& map_a
 
 int few_tile_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
 
-int few_split(int sm_count, int N, int k_blocks) {
-    const int blocks = (N + 127) / 128;
-    int split = 1;
-    while (split < kFewSplitMax && blocks * split * 2 <= 2 * sm_count && split * 4 <= k_blocks) split *= 2;
-    return split;
-}
-
-cudaError_t few_launch(bool int8, int split, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream) {
+cudaError_t few_launch(bool int8, int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream) {
     const int rows = few_tile_rows(p.M);
-    if (int8) return rows == 16 ? launch<true, 16>(split, map_b, map_a, p, stream) : rows == 32 ? launch<true, 32>(split, map_b, map_a, p, stream) : launch<true, 64>(split, map_b, map_a, p, stream);
-    return rows == 16 ? launch<false, 16>(split, map_b, map_a, p, stream) : rows == 32 ? launch<false, 32>(split, map_b, map_a, p, stream) : launch<false, 64>(split, map_b, map_a, p, stream);
+    const auto go = [&](auto f) { return f(sm_count, map_b, map_a, p, stream); };
+    if (int8) return rows == 16 ? go(launch<true, 16>) : rows == 32 ? go(launch<true, 32>) : go(launch<true, 64>);
+    return rows == 16 ? go(launch<false, 16>) : rows == 32 ? go(launch<false, 32>) : go(launch<false, 64>);
 }
 
 }  // namespace sl8

@@ -8,7 +8,9 @@
 
 namespace sl8 {
 
-constexpr int kFewRowsMax = 64;            // rows of A these kernels take
+// Whether these kernels take a product.  Up to 16 rows always; up to 32 and 64 where K is deep enough that the tiles of 64 columns,
+// which do not share it out, take longer.
+inline bool few_rows(long long M, int K) { return M <= 16 || (M <= 32 && K > 1024) || (M <= 64 && K > 2944); }
 constexpr int kFewSplitMax = 8;            // CTAs of a cluster, each with a share of K
 
 struct FewParams {
@@ -21,15 +23,15 @@ struct FewParams {
     void* D;
     long long ldd;
     unsigned flags;
+    int stages;                      // set by few_launch: depth of the operand ring,
+    int share;                       // and rows that each CTA of a cluster finishes (a multiple of four)
     unsigned wait_budget_us;
     uint32_t* status;
 };
 
-// CTAs that share the K of one block of 128 columns.
-int few_split(int sm_count, int N, int k_blocks);
 // Rows of the tile that M rows of A take: the box of map_a.
 int few_tile_rows(int M);
 // map_b: boxes of 128 rows x 128 bytes of B; map_a: few_tile_rows(M) x 128 bytes of A.
-cudaError_t few_launch(bool int8, int split, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream);
+cudaError_t few_launch(bool int8, int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream);
 
 }  // namespace sl8

@@ -358,14 +358,27 @@ def test_a_row_that_is_no_number_stays_alone(engine, M):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("codes", [I8, F8])
-def test_rows_do_not_depend_on_their_neighbours(engine, codes):
-    """The same rows alone and among others, on the kernels for few rows: bit for bit (K is shared out by N and K alone)."""
-    A, sa = operand(64, 2000, codes, 1)
-    B, sb = operand(400, 2000, codes, 2)
-    whole = engine.linear_scaled(A, B, sa, sb)
-    for lo, hi in ((0, 1), (5, 6), (10, 26), (20, 50), (63, 64)):
-        assert torch.equal(engine.linear_scaled(A[lo:hi], B, sa[lo:hi].clone(), sb), whole[lo:hi])
+@pytest.mark.parametrize("N,K", [(400, 2000), (1152, 4304), (272, 100)])
+def test_rows_do_not_depend_on_their_neighbours(engine, N, K):
+    """int8: the same rows alone and among others are the same bit for bit, whichever kernel the number of rows calls for."""
+    A, sa = operand(300, K, I8, 1)
+    B, sb = operand(N, K, I8, 2)
+    bias = torch.randn((N,), generator=gen(4), device=DEV)
+    for flags in (0, L.SL8_FLAG_GELU):
+        whole = engine.linear_scaled(A, B, sa, sb, bias, flags=flags)
+        for lo, hi in ((0, 1), (5, 6), (10, 26), (20, 50), (63, 64), (100, 164), (10, 139)):
+            assert torch.equal(engine.linear_scaled(A[lo:hi], B, sa[lo:hi].clone(), sb, bias, flags=flags), whole[lo:hi])
+
+
+@pytest.mark.gpu
+def test_the_same_call_twice(engine):
+    """e4m3 sums are fp32: the order of their parts is fixed."""
+    for M in (1, 16, 30, 64, 500):
+        A, sa = operand(M, 4304, F8, 1)
+        B, sb = operand(1152, 4304, F8, 2)
+        first = engine.linear_scaled(A, B, sa, sb)
+        for _ in range(5):
+            assert torch.equal(engine.linear_scaled(A, B, sa, sb), first)
 
 
 # ----------------------------------------------------------------------------- together
