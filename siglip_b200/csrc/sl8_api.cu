@@ -11,7 +11,6 @@
 
 #include "sl8_internal.h"
 #include "sl8_dispatch_table.h"
-#include "sl8_few.h"
 
 namespace {
 
@@ -281,7 +280,7 @@ int run_few(sl8_handle_t h, const Problem& q, cudaStream_t stream) {
                    (unsigned long long)q.lda, 128, (unsigned)sl8::few_tile_rows(p.M), CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
     if (rc != SL8_OK) return rc;
     h->last_grid = 0;        // these kernels write no trace records
-    const cudaError_t e = sl8::few_launch(q.op == kOpInt8, h->sm_count, map_b, map_a, p, stream);
+    const cudaError_t e = sl8::few_launch(h->few, q.op == kOpInt8, h->sm_count, map_b, map_a, p, stream);
     return e == cudaSuccess ? SL8_OK : fail_cuda(h, e, "kernel launch");
 }
 

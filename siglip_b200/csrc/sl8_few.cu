@@ -16,24 +16,23 @@ struct FewTraits {
     static constexpr int W_BYTES = 128 * 128, STAGE_BYTES = W_BYTES + ROWS * 128;
     static constexpr int SUM_BYTES = (ROWS < 4 * kFewSplitMax ? 4 * kFewSplitMax : ROWS) * 128 * 4;   // partial sums of the rows this CTA finishes
     static constexpr int VEC_FLOATS = 2 * 128 + ROWS;                       // column scales, bias, row scales
-    // The ring: deep where every CTA has an SM of its own, else such that two CTAs fit one.
-    static constexpr int DEEP = ROWS == 64 ? 7 : 8, HALF = ROWS == 16 ? 5 : ROWS == 32 ? 4 : 3;
+    // The ring: deep where every CTA has an SM of its own, else such that two CTAs fit one (of 128 rows, one).
+    static constexpr int DEEP = ROWS == 128 ? 5 : ROWS == 64 ? 7 : 8, HALF = ROWS == 16 ? 5 : ROWS == 32 ? 4 : ROWS == 64 ? 3 : 5;
     static constexpr int smem_bytes(int stages) { return 1024 + stages * STAGE_BYTES + SUM_BYTES + 4 * VEC_FLOATS + 256; }
-    static_assert(smem_bytes(DEEP) <= 232448 && 2 * (smem_bytes(HALF) + 1024) <= 228 * 1024, "one and two CTAs per SM");
+    static_assert(smem_bytes(DEEP) <= 232448 && (ROWS == 128 || 2 * (smem_bytes(HALF) + 1024) <= 228 * 1024), "one and two CTAs per SM");
     static_assert(2 * DEEP + 1 <= 32 && 16 * DEEP + 16 <= 256, "a barrier per lane; room for them");
     static constexpr int TMEM_COLS = ROWS < 32 ? 32 : ROWS;
     static_assert(STAGE_BYTES % 1024 == 0, "every operand tile starts on a swizzle-atom boundary");
 };
 
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 256;        // two warps for each quarter of the tensor memory's lanes
 
 __device__ __forceinline__ void st_cluster_16(uint32_t addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&v)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
                  : "r"(taddr)
                  : "memory");
 }
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     }
     if (warp >= 2) {
         // while the operands come: what the sums are multiplied with
-        for (int i = threadIdx.x - 64; i < 128; i += 64) {
+        for (int i = threadIdx.x - 64; i < 128; i += kFewThreads - 64) {
             float col_scale = 0.0f, bias = 0.0f;
             if (n0 + i < p.N) {
                 col_scale = ld_f32(p.col_scales + n0 + i);
@@ -144,14 +143,15 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
             vec[i] = col_scale;
             vec[128 + i] = bias;
         }
-        for (int i = threadIdx.x - 64; i < p.M; i += 64) vec[256 + i] = ld_f32(p.row_scales + i);
+        for (int i = threadIdx.x - 64; i < p.M; i += kFewThreads - 64) vec[256 + i] = ld_f32(p.row_scales + i);
     }
     __syncthreads();
     const bool ok = __all_sync(0xffffffffu, wait_bar<true>(done, 0, wc, ST_EPI_TMEM_FULL_WAIT, 0)) != 0;
     tc_fence_after();
 
-    const int n = n0 + static_cast<int>(threadIdx.x);       // this thread's output channel: TMEM lane threadIdx.x
-    const float col_scale = vec[threadIdx.x], bias = vec[128 + threadIdx.x];
+    const int ch = threadIdx.x & 127, half = threadIdx.x >> 7;       // this thread's output channel (TMEM lane), and which of the rows it takes
+    const int n = n0 + ch;
+    const float col_scale = vec[ch], bias = vec[128 + ch];
     const auto sum_of = [](float a, float b) { return I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b; };
     const auto number = [](float sum) { return I8 ? __int2float_rn(__float_as_int(sum)) : sum; };
     // rows m .. m + 3 of this channel, as far as there are so many
@@ -170,46 +170,47 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
                 if (m + i < p.M) *d = __float2bfloat16_rn(y[i]);
         }
     };
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    constexpr int CHUNK = 16;
-    if (split == 1) {
-        if (ok) {
+    const uint32_t t_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // the rows of this half, eight or sixteen at a time: f(first row, sums)
+    constexpr int CHUNK = ROWS == 16 ? 8 : 16;
+    const auto chunks = [&](auto&& f) {
 #pragma unroll 1
-            for (int c = 0; c < p.M; c += CHUNK) {
-                float v[CHUNK];
-                tmem_ld_32x16(t_row + c, v);
-                tmem_ld_wait();
+        for (int c = half * CHUNK; c < p.M; c += 2 * CHUNK) {
+            float v[CHUNK];
+#pragma unroll
+            for (int i = 0; i < CHUNK; i += 8) tmem_ld_32x8(t_row + c + i, v + i);
+            tmem_ld_wait();
+            f(c, v);
+        }
+    };
+    if (split == 1) {
+        if (ok)
+            chunks([&](int c, const float* v) {
 #pragma unroll
                 for (int i = 0; i < CHUNK; i += 4)
                     if (c + i < p.M) finish4(c + i, v[i], v[i + 1], v[i + 2], v[i + 3]);
-            }
-        }
+            });
     } else {
         // Each rank of the cluster finishes `share` rows, a multiple of four: it gets their sums from every rank.
         const int share = p.share, own = static_cast<int>(rank) * share;
         cluster_wait();
-        if (ok) {
-            int owner = 0, at = 0;
-#pragma unroll 1
-            for (int c = 0; c < p.M; c += CHUNK) {
-                float v[CHUNK];
-                tmem_ld_32x16(t_row + c, v);
-                tmem_ld_wait();
+        if (ok)
+            chunks([&](int c, const float* v) {
+                int owner = c / share, at = c - owner * share;
 #pragma unroll
                 for (int i = 0; i < CHUNK; i += 4)
                     if (c + i < p.M) {
-                        st_cluster_16(map_to_cta(sums + ((rank * 128 + threadIdx.x) * share + at) * 4, owner), v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        st_cluster_16(map_to_cta(sums + ((rank * 128 + ch) * share + at) * 4, owner), v[i], v[i + 1], v[i + 2], v[i + 3]);
                         at += 4;
                         if (at == share) at = 0, owner++;
                     }
-            }
-        }
+            });
         __syncwarp();
         cluster_arrive();
         if (own < p.M) {               // (a CTA that finishes no row is written to by none)
             cluster_wait();
-            const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + threadIdx.x * share;
-            for (int i = 0; i < share && own + i < p.M; i += 4) {
+            const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + ch * share;
+            for (int i = 4 * half; i < share && own + i < p.M; i += 8) {
                 float4 s = *reinterpret_cast<const float4*>(mine + i);
                 for (uint32_t q = 1; q < split; q++) {
                     const float4 o = *reinterpret_cast<const float4*>(mine + q * 128 * share + i);
@@ -235,50 +236,75 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
 }
 
 // CTAs that share the K of one block of 128 columns: as many as give each SM one, with at least one and a half k-blocks for each.
+int blocks_of(int N) { return N / 128 + (N % 128 != 0 ? 1 : 0); }
 int few_split(int sm_count, int N, int k_blocks) {
-    const int blocks = (N + 127) / 128;
+    const int blocks = blocks_of(N);
     int split = 1;
     while (split < kFewSplitMax && blocks * split * 2 <= sm_count && split * 3 <= k_blocks) split *= 2;
     return split;
 }
 
 template <bool I8, int ROWS>
-cudaError_t launch(int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, FewParams p, cudaStream_t stream) {
-    const int split = few_split(sm_count, p.N, p.k_blocks);
+cudaError_t launch(FewKernelState& state, int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, FewParams p, cudaStream_t stream) {
+    int split = few_split(sm_count, p.N, p.k_blocks);
     using T = FewTraits<ROWS>;
     const auto kernel = few_rows_kernel<I8, ROWS>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::smem_bytes(T::DEEP));
-    if (e != cudaSuccess) return e;
-    const int ctas = (p.N + 127) / 128 * split, most = (p.k_blocks + split - 1) / split;
-    p.stages = ctas <= sm_count ? T::DEEP : T::HALF;
-    if (p.stages > most) p.stages = most;            // (a short ring leaves room for the next kernel's CTAs)
-    p.share = (p.M + 4 * split - 1) / (4 * split) * 4;
+    if (!state.attr_set) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::smem_bytes(T::DEEP));
+        if (e != cudaSuccess) return e;
+        state.attr_set = true;
+    }
+    const int blocks = blocks_of(p.N);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
     cfg.blockDim = dim3(kFewThreads, 1, 1);
-    cfg.dynamicSmemBytes = static_cast<size_t>(T::smem_bytes(p.stages));
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    const auto shape = [&](int stages) {
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks * split), 1, 1);
+        cfg.dynamicSmemBytes = static_cast<size_t>(T::smem_bytes(stages));
+        attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    };
+    // How many clusters of CTAs with the deep ring are resident at once: fewer than the SMs would give room to, because a cluster has
+    // to find its SMs in one part of the chip (of eight: 15).
+    const auto resident = [&]() {
+        int& fit = state.clusters[split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3];
+        if (fit == 0) {
+            shape(T::DEEP);
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess || fit < 1) {
+                (void)cudaGetLastError();
+                fit = sm_count / split;
+            }
+        }
+        return fit;
+    };
+    // (of 64 and 128 rows a second round of clusters costs more than a share of K twice as long: 64 x 8 192 -> 2 048 11.2 -> 9.8 us)
+    while (ROWS >= 64 && split > 1 && blocks > resident()) split /= 2;
+    const int most = (p.k_blocks + split - 1) / split;
+    p.stages = blocks <= resident() ? T::DEEP : T::HALF;
+    if (p.stages > most) p.stages = most;            // (a short ring leaves room for the next kernel's CTAs)
+    shape(p.stages);
     cfg.numAttrs = 2;
+    p.share = (p.M + 4 * split - 1) / (4 * split) * 4;
     return cudaLaunchKernelEx(&cfg, kernel, map_b, map_a, p);
 }
 
 }  // namespace
 
-int few_tile_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+int few_tile_rows(int M) { return M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128; }
 
-cudaError_t few_launch(bool int8, int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream) {
+cudaError_t few_launch(FewState& state, bool int8, int sm_count, const CUtensorMap& map_b, const CUtensorMap& map_a, const FewParams& p, cudaStream_t stream) {
     const int rows = few_tile_rows(p.M);
-    const auto go = [&](auto f) { return f(sm_count, map_b, map_a, p, stream); };
-    if (int8) return rows == 16 ? go(launch<true, 16>) : rows == 32 ? go(launch<true, 32>) : go(launch<true, 64>);
-    return rows == 16 ? go(launch<false, 16>) : rows == 32 ? go(launch<false, 32>) : go(launch<false, 64>);
+    FewKernelState& kernel = state.kernel[int8 ? 1 : 0][rows == 16 ? 0 : rows == 32 ? 1 : rows == 64 ? 2 : 3];
+    const auto go = [&](auto f) { return f(kernel, sm_count, map_b, map_a, p, stream); };
+    if (int8) return rows == 16 ? go(launch<true, 16>) : rows == 32 ? go(launch<true, 32>) : rows == 64 ? go(launch<true, 64>) : go(launch<true, 128>);
+    return rows == 16 ? go(launch<false, 16>) : rows == 32 ? go(launch<false, 32>) : rows == 64 ? go(launch<false, 64>) : go(launch<false, 128>);
 }
 
 }  // namespace sl8

@@ -10,6 +10,7 @@
 #include <string>
 
 #include "../../include/siglip_fp8.h"
+#include "sl8_few.h"
 #include "sl8_variants.h"
 
 #define SL8_API extern "C" __attribute__((visibility("default")))
@@ -67,6 +68,7 @@ struct sl8_context {
     unsigned wait_budget_us = 2000000;
     bool smem_attr_set[SL8_NUM_VARIANTS][sl8::K_COUNT] = {};
     int max_clusters[SL8_NUM_VARIANTS][sl8::K_COUNT] = {};
+    sl8::FewState few;
     std::mutex mu;          // the handle's state during one launch (map cache, attributes, error text)
     std::mutex pipe_mu;     // the host-operand pipeline during one *_host call (taken before mu)
     std::string err;

@@ -620,6 +620,7 @@ int run_rows(sl8_handle_t h, const RowArgs& a, sl8_stream_t stream, const char* 
     return e == cudaSuccess ? SL8_OK : sl8_fail_cuda(h, e, what);
 }
 
+constexpr int kMostColumns = 1 << 30;       // columns are counted in steps of 32 bits
 bool element_aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == SL8_DT_F32 ? 3u : 1u)) == 0; }
 bool float_aligned(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
@@ -632,6 +633,7 @@ SL8_API int sl8_quantize_rows(sl8_handle_t h, const void* x, int dtype, int64_t 
         return sl8_fail(h, SL8_ERR_INVALID_VALUE, "bad quantize_rows arguments");
     if (dtype != SL8_DT_F32 && dtype != SL8_DT_BF16) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "unknown dtype");
     if (code_type != SL8_CODE_INT8 && code_type != SL8_CODE_E4M3) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "unknown code type");
+    if (cols > kMostColumns) return sl8_fail(h, SL8_ERR_UNSUPPORTED, "more than 2^30 columns");
     if (!element_aligned(x, dtype) || !float_aligned(row_scales)) return sl8_fail(h, SL8_ERR_ALIGNMENT, "x and row_scales must be aligned to their elements");
     RowArgs a = {};
     a.x = x; a.ld = ld;
@@ -649,6 +651,7 @@ SL8_API int sl8_rmsnorm_quantize(sl8_handle_t h, const void* x, int dtype, int64
         return sl8_fail(h, SL8_ERR_INVALID_VALUE, "bad rmsnorm arguments");
     if (dtype != SL8_DT_F32 && dtype != SL8_DT_BF16) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "unknown dtype");
     if (code_type != SL8_CODE_INT8 && code_type != SL8_CODE_E4M3) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "unknown code type");
+    if (cols > kMostColumns) return sl8_fail(h, SL8_ERR_UNSUPPORTED, "more than 2^30 columns");
     if ((residual == nullptr) != (sum == nullptr)) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "residual and sum come together");
     if (residual && (ld_res < cols || ld_sum < cols)) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "ld_res / ld_sum smaller than cols");
     if (row_scales && scale) return sl8_fail(h, SL8_ERR_INVALID_VALUE, "a scale is given, or written for each row");

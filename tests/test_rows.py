@@ -274,7 +274,7 @@ def check_linear(got, A, B, sa, sb, bias, gelu, codes):
 
 SHAPES = [(1, 16, 1), (1, 1152, 4304), (2, 48, 16), (3, 128, 31), (8, 144, 128), (15, 272, 129), (16, 4304, 1152), (17, 256, 300), (31, 1168, 588), (32, 64, 2048),
           (33, 400, 1155), (63, 128, 640), (64, 1152, 4304), (65, 1152, 300), (100, 16, 32), (127, 48, 33), (128, 112, 4304), (129, 240, 257), (300, 336, 1155),
-          (729, 1152, 588), (257, 4304, 100), (1000, 592, 999)]
+          (65, 144, 12288), (128, 400, 12333), (97, 2048, 12400), (10, 2048, 8192), (50, 2064, 8000), (729, 1152, 588), (257, 4304, 100), (1000, 592, 999)]
 
 
 @pytest.mark.gpu
@@ -522,6 +522,27 @@ def test_a_wait_that_runs_out(monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [1152, 1153, 4304])
+def test_a_row_that_never_comes(monkeypatch, cols):
+    """The same of the kernels that bring rows into shared memory."""
+    from siglip_b200 import Engine
+    monkeypatch.setenv("SL8_TEST_DROP_B", "1")
+    dropping = Engine(0)
+    monkeypatch.delenv("SL8_TEST_DROP_B")
+    x = activations(9000, cols, BF16, 1)
+    dropping.set_wait_budget_us(3000)
+    dropping.quantize_rows(x)
+    with pytest.raises(L.SL8Error) as e:
+        dropping.device_status()
+    assert e.value.code == L.SL8_ERR_DEVICE_TIMEOUT and dropping.last_status_detail[0] == 7 and dropping.last_status_detail[2] == 1
+    dropping.close()
+    with Engine(0) as e:
+        q, s = e.quantize_rows(x)
+        e.device_status()
+        assert torch.equal(q[:64], e.quantize_rows(x[:64])[0])
+
+
+@pytest.mark.gpu
 def test_the_library_refuses(engine):
     """Straight at the C ABI: what the Python checks would stop."""
     lib, h = engine._lib, engine._h
@@ -534,6 +555,7 @@ def test_the_library_refuses(engine):
     for bad in (dict(x=None), dict(o=None), dict(s=None), dict(dt=2), dict(t=2), dict(t=-1), dict(r=0), dict(c=0), dict(ld=63), dict(lo=63)):
         assert quant(**bad) == L.SL8_ERR_INVALID_VALUE, bad
     assert quant(h=None) == L.SL8_ERR_INVALID_VALUE
+    assert quant(r=1, c=(1 << 30) + 8, ld=1 << 31, lo=1 << 31) == L.SL8_ERR_UNSUPPORTED
     for bad in (dict(x=p(x, 1)), dict(s=p(sc, 2))):
         assert quant(**bad) == L.SL8_ERR_ALIGNMENT, bad
     norm = lambda **k: lib.sl8_rmsnorm_quantize(*({"h": h, "x": p(x), "dt": 1, "r": 4, "c": 64, "ld": 64, "res": None, "lr": 0, "sum": None, "ls": 0, "g": None, "eps": 1e-6, "t": 1,  # noqa: E731
