@@ -113,6 +113,8 @@ int cheapest_variant(sl8_handle_t h, CostClass cls, int slot, long long M, int N
 
 int pick_variant(sl8_handle_t h, int op, int out_dtype, long long M, int N, int K, unsigned flags) {
     const int slot = kernel_slot(op, out_dtype);
+    // (1 976 points from 144 to 8 192 wide and 96 to 46 656 rows, int8 and e4m3: these constants pick 0.7 - 1.4 % off the fastest on average,
+    // 17 % at worst from 512 columns on; constants fitted to them would pick 0.8 and 0.7 %)
     if (sl8::op_scaled(op)) return cheapest_variant(h, (flags & SL8_FLAG_NO_ACTIVATION) ? COST_NONE : COST_GELU, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_NO_ACTIVATION)) return cheapest_variant(h, COST_NONE, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_GELU_HW_TANH)) return cheapest_variant(h, COST_TANH, slot, M, N, K);

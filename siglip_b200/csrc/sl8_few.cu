@@ -1,10 +1,13 @@
 // sl8_few.cu -- sl8_linear_scaled for few rows of A: one token each of some sequences.
 //
-// The product is that of the weights' bytes with hardly anything, so it is turned round: 128 rows of B are the M of a
-// tcgen05.mma, the rows of A (16, 32 or 64, what is missing read as zeros) its N, and a CTA brings 16 KiB of weights per k-block
-// for 2 - 8 KiB of activations.  K is shared by the CTAs of a cluster, because the weights of few output channels would
-// otherwise come through few SMs; their partial sums meet in shared memory (exact for int8, in the order of the ranks for
-// e4m3: the same result every time), and each CTA finishes a share of the rows.
+// What takes time is the weights' way in, so the product is turned round: 128 rows of B are the M of a tcgen05.mma, the rows of A (16,
+// 32, 64 or 128, what is missing read as zeros) its N, and a CTA brings 16 KiB of weights per k-block for 2 - 16 KiB of
+// activations.  K is shared out to the CTAs of a cluster, because the weights of few output channels would otherwise come through few
+// SMs (1 x 4 304 -> 1 152: 8 CTAs 3.8 us, 4 4.4, 2 6.0).  Each CTA writes its partial sums into the shared memory of the one that
+// finishes the row, four rows at a time, and one cluster barrier stands between that and the adding up: exact for int8, in the order of
+// the ranks for e4m3, so the same result every time.  (Read from there instead, with a barrier on either side: 4.4 us.)
+// Bound by the weights' bytes where there are many (32 768 x 4 096, 134 MB: 22.4 us, 6.0 TB/s; 8 192 x 8 192 13.3 us, 5.0), by the way
+// of one k-block through all of it where there are few: about 2.8 us from launch to launch (768 x 768).
 #include "sl8_kernel.cuh"
 #include "sl8_few.h"
 
@@ -284,6 +287,7 @@ cudaError_t launch(FewKernelState& state, int sm_count, const CUtensorMap& map_b
         }
         return fit;
     };
+    // The deep ring where all clusters are resident at once with it (1 x 4 096 -> 14 336 12.8 us with two CTAs per SM, 11.7 so).
     // (of 64 and 128 rows a second round of clusters costs more than a share of K twice as long: 64 x 8 192 -> 2 048 11.2 -> 9.8 us)
     while (ROWS >= 64 && split > 1 && blocks > resident()) split /= 2;
     const int most = (p.k_blocks + split - 1) / split;

@@ -212,8 +212,10 @@ __device__ __forceinline__ Scaling scaling(const RowArgs& a, const Stats& s, flo
 }
 
 // A row by the threads of a block (or, WARP, of a warp), CH times eight elements each: read once and held in registers, everything
-// asked for before the first of it is used; statistics in fp32, four partial sums a thread.  Bound by the bytes of x, the
-// residual, their sum and the codes.
+// asked for before the first of it is used; statistics in fp32, four partial sums a thread.  For one wave of rows: bound by one trip
+// to memory and the launch (one row of 1 152 bf16 with a residual 1.7 us, 8 rows of 4 304 1.5; 5 003 x 1 152 by warps 5.4).  Gamma
+// comes through shared memory while the first row is on its way: kept in registers it costs a third of the warps (fp32 46 656 x 1 152
+// 80 us, 65 so).
 constexpr int kWarpRowThreads = 128;
 template <typename T, bool NORM, bool VEC, int CH, bool WARP>
 __global__ void __launch_bounds__(WARP ? kWarpRowThreads : CH == 1 ? 1024 : 512) row_kernel(const RowArgs a) {
@@ -329,6 +331,13 @@ __device__ __forceinline__ void shared_values(float (&v)[8], const T* p, int lef
     }
 }
 
+// The same for many rows: each block (or, WARP, warp) has a ring of two slots in shared memory and asks for a row, one bulk copy for x and
+// one for the residual, as soon as the one two before it has been read, so that there is always a row on its way and the registers
+// hold one only.  Bound by the bytes: 46 656 x 4 304 bf16 -> int8 92 us, the copy rate of this memory (rows in registers 115);
+// RMS norm of 16 384 x 4 096 with a residual 77 us, 6.1 TB/s (84); 46 656 x 1 152 fp32 -> e4m3 49 us, 5.5 TB/s (65).  Three slots
+// were slower nearly everywhere (16 384 x 4 096 81 us: fewer blocks fit).
+// Rows on any address: the copy takes the 16-byte granules that the row touches, and lanes read consecutive elements from there.  5 003 x 4 305
+// bf16 17.8 us, 3.6 TB/s (from memory, lane by lane, 52: a warp's loads of 64 bytes do not keep enough in flight); the codes go out byte by byte.
 constexpr int kSlots = 2;
 __host__ __device__ constexpr int gamma_bytes(bool given, int cols) { return given ? (cols + 255) / 256 * 1024 : 0; }
 template <typename T, bool NORM, bool VEC, int CH, bool WARP>
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRowThreads : 512) row_stream_kerne
     }
 }
 
-// Rows too long for the registers of a block: read twice, statistics first.  The sum is written the second time only, because it may
+// Rows too long for the registers of a block, or for its ring: read twice, statistics first.  The sum is written the second time only, because it may
 // lie where the second reading still has to find x or the residual.
 constexpr int kLongThreads = 512;
 template <typename T, bool NORM, bool VEC>
@@ -582,8 +591,12 @@ cudaError_t stream_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     return sl8_launch_chained(kernel, static_cast<unsigned>(want < once * waves ? want : once * waves), threads, bytes, s, a, span);
 }
 
-// Few rows: a block each, one trip to memory; from then on a warp each while rows are short, as long as there is hardly a second row
-// for a warp; then, and where rows start on odd addresses, the ring in shared memory.
+// Up to ten rows per SM: a block each, one trip to memory (1 500 x 4 304 bf16 -> int8 5.9 us, ring 6.5); with all eight elements of a
+// thread's at once while 256 threads do (norm of one row of 1 152 1.74 us, 1.95 with three times eight), with three from there on (729 x 4 304
+// 3.6 us, 5.4 with one).  Up to forty, where rows are short: a warp each (norm of 5 003 x 1 152 10.3 us, ring 10.9).  Then the ring, by
+// warps while rows are short, by blocks of three times eight elements a thread (100 000 x 512 57 us by warps, 64 by blocks; 20 000 x
+// 2 048 50 either way; 46 656 x 4 304 92, 94 with four, 96 with two), and rows on odd addresses from the tenth row per SM (norm of
+// 5 003 x 1 155 15.5 us, in registers 30).
 template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     const bool few = a.rows <= 10ll * sm_count;

@@ -233,6 +233,94 @@ def test_rmsnorm_pitched_operands(engine):
         assert (whole[mask] == 9.0).all()
 
 
+# ----------------------------------------------------------------------------- many rows: rings in shared memory, several rows per warp or block
+# (rows, columns, elements ahead of the first row, pitch): whole vectors and not, each width that has a kernel of its own
+MANY = [(6100, 8, 0, 8), (6001, 256, 8, 272), (6011, 504, 0, 512), (6003, 768, 0, 768), (6007, 1152, 16, 1160), (12345, 1280, 0, 1280), (1481, 1288, 8, 1296), (2999, 2048, 0, 2048),
+        (1777, 4304, 0, 4304), (1483, 8192, 0, 8192), (1482, 12288, 0, 12288), (1490, 12296, 8, 12304), (1485, 16384, 0, 16384), (1481, 16392, 0, 16392),
+        (1700, 9, 1, 9), (1600, 13, 0, 17), (1503, 255, 3, 255), (1502, 256, 1, 257), (2001, 333, 0, 333), (1600, 511, 5, 600), (1555, 767, 0, 768), (1500, 769, 7, 769),
+        (3001, 1155, 0, 1155), (1490, 2047, 1, 2049), (1481, 2050, 0, 2050), (1482, 4305, 3, 4305), (1483, 12287, 0, 12287), (1484, 12290, 1, 12290), (1481, 16383, 0, 16383),
+        (1481, 16385, 1, 16385)]
+
+
+def surrounded(rows, cols, ahead, pitch, dtype, seed, std=1.0):
+    """Rows inside a buffer that is NaN everywhere else."""
+    x = activations(rows, cols, dtype, seed, std)
+    buf = torch.full((ahead + (rows - 1) * pitch + cols + 5,), math.nan, dtype=dtype, device=DEV)
+    view = torch.as_strided(buf, (rows, cols), (pitch, 1), ahead)
+    view.copy_(x)
+    return view, buf
+
+
+def fenced_codes(rows, cols, pitch):
+    codes = torch.full((16 + (rows + 1) * pitch,), 85, dtype=U8, device=DEV)
+    written = torch.zeros_like(codes, dtype=torch.bool)
+    torch.as_strided(written, (rows, cols), (pitch, 1), 16).fill_(True)
+    return codes, torch.as_strided(codes, (rows, cols), (pitch, 1), 16), written
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols,ahead,pitch", MANY)
+def test_quantize_many_rows_bit_for_bit(engine, dtype, rows, cols, ahead, pitch):
+    x, _ = surrounded(rows, cols, ahead, pitch, dtype, rows + cols)
+    x[rows // 2] = 0.0
+    for codes in (I8, F8):
+        flat, out, written = fenced_codes(rows, cols, (cols + 15) // 16 * 16 + 16)
+        q, scales = engine.quantize_rows(x, codes, out=out.view(codes))
+        engine.device_status()
+        amax = x.float().abs().amax(1)
+        top = torch.tensor(TOP[codes], device=DEV)
+        assert torch.equal(scales, torch.where(amax == 0, torch.ones_like(amax), amax / top))
+        k = torch.where(amax == 0, torch.ones_like(amax), top / amax)[:, None]
+        for r in range(0, rows, 2048):          # (products of two fp32 numbers are exact in 64 bits)
+            v = x[r:r + 2048].float()
+            want = torch.round(v.double() * k[r:r + 2048].double()).to(I8) if codes == I8 else (v * k[r:r + 2048]).clamp(-448.0, 448.0).to(F8)
+            assert torch.equal(q[r:r + 2048].view(U8), want.view(U8)), r
+        assert (flat[~written] == 85).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols,ahead,pitch", MANY)
+def test_rmsnorm_of_many_rows(engine, dtype, rows, cols, ahead, pitch):
+    """Against 64 bits: with a residual of another pitch into a third buffer, and without; the sum in place."""
+    x, whole = surrounded(rows, cols, ahead, pitch, dtype, rows + cols)
+    r, _ = surrounded(rows, cols, ahead + 8, pitch + 8, dtype, rows + cols + 1, std=3.0)
+    g = 1 + 0.2 * torch.randn((cols,), generator=gen(3), device=DEV)
+    rel = norm_error(cols)
+    for residual, codes in ((r, I8), (None, F8), (r, "static")):
+        flat, out, written = fenced_codes(rows, cols, (cols + 15) // 16 * 16)
+        if codes == "static":
+            q, summed = engine.rmsnorm_quantize(x, g, 1e-5, torch.tensor([0.02], device=DEV), residual=residual, out=out)
+            scales, kind = torch.full((rows,), 0.02, device=DEV), F8
+        else:
+            q, scales, *rest = engine.rmsnorm_quantize_rows(x, g, 1e-5, codes, residual=residual, out=out.view(codes))
+            summed, kind = (rest + [None])[0], codes
+        engine.device_status()
+        for lo in range(0, rows, 2048):
+            part = slice(lo, lo + 2048)
+            y = norm64(x[part], None if residual is None else residual[part], g, 1e-5)
+            s = scales[part].double()[:, None]
+            if codes == "static":
+                y = y.clamp(-448 * 0.02, 448 * 0.02)
+            else:
+                want = y.abs().amax(1, keepdim=True) / TOP[codes]
+                assert ((s - want).abs() <= want * (rel + 2.0 ** -23)).all()
+            half = (s / 2).expand_as(y) if kind == I8 else torch.maximum(y.abs() * (1 + 2 * rel) * 2.0 ** -4, s * 2.0 ** -10)
+            value = (q[part] if kind == I8 else q[part].view(F8)).double() * s
+            assert ((value - y).abs() <= half + y.abs() * 2 * (rel + 2.0 ** -22)).all(), lo
+        assert (flat[~written] == 85).all()
+        if residual is not None:
+            assert torch.equal(summed, (x.float() + residual.float()).to(dtype))
+    want = engine.rmsnorm_quantize_rows(x, g, residual=r)
+    before = whole.clone()
+    got = engine.rmsnorm_quantize_rows(x, g, residual=r, summed=x)
+    assert got[2] is x and all(torch.equal(a, b) for a, b in zip(got, want))
+    inside = torch.zeros_like(whole, dtype=torch.bool)
+    torch.as_strided(inside, (rows, cols), (pitch, 1), ahead).fill_(True)
+    assert torch.equal(whole[~inside].isnan(), before[~inside].isnan())
+
+
 # ----------------------------------------------------------------------------- the product
 def operand(rows, cols, codes, seed, pitch=None):
     g = gen(seed)
@@ -379,6 +467,30 @@ def test_the_same_call_twice(engine):
         first = engine.linear_scaled(A, B, sa, sb)
         for _ in range(5):
             assert torch.equal(engine.linear_scaled(A, B, sa, sb), first)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(engine):
+    """Rows that lie more than 2^31 elements apart from first to last, read and written."""
+    cols = 1152
+    for rows, pitch in ((3, 1 << 30), (1500, 1 << 21), (1500, (1 << 21) + 1)):
+        buf = torch.empty(((rows - 1) * pitch + cols,), dtype=BF16, device=DEV)
+        x = torch.as_strided(buf, (rows, cols), (pitch, 1))
+        x.copy_(activations(rows, cols, BF16, 1))
+        assert all(torch.equal(a, b) for a, b in zip(engine.quantize_rows(x), engine.quantize_rows(x.contiguous())))
+        want = engine.rmsnorm_quantize_rows(x.contiguous(), residual=x.contiguous())
+        got = engine.rmsnorm_quantize_rows(x, residual=x, summed=x)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+        del buf, x, got
+    for M, pitch in ((16, 1 << 28), (130, 1 << 25)):
+        A, sa = operand(M, 256, I8, 1)
+        B, sb = operand(144, 256, I8, 2)
+        buf = torch.empty(((M - 1) * pitch + 144,), dtype=BF16, device=DEV)
+        D = torch.as_strided(buf, (M, 144), (pitch, 1))
+        engine.linear_scaled(A, B, sa, sb, out=D)
+        assert torch.equal(D, engine.linear_scaled(A, B, sa, sb))
+        del buf, D
+    engine.device_status()
 
 
 # ----------------------------------------------------------------------------- together
