@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     extern __shared__ uint8_t few_smem[];
     const uint32_t raw = smem_u32(few_smem);
     const uint32_t base = (raw + 1023u) & ~1023u;
-    const uint32_t sums = base + p.stages * T::STAGE_BYTES;                            // [rank][128][rows of this CTA]
+    const uint32_t sums = base + p.stages * T::STAGE_BYTES;                            // [rank][four rows of this CTA][128][4]: 16 bytes per thread, side by side
     float* const vec = reinterpret_cast<float*>(few_smem + (sums - raw) + T::SUM_BYTES);  // column scales, bias, row scales
     uint8_t* const bar_ptr = reinterpret_cast<uint8_t*>(vec + T::VEC_FLOATS);
     const uint32_t full0 = sums + T::SUM_BYTES + 4 * T::VEC_FLOATS, empty0 = full0 + 8 * p.stages, done = empty0 + 8 * p.stages;
@@ -199,24 +199,23 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
         cluster_wait();
         if (ok)
             chunks([&](int c, const float* v) {
-                int owner = c / share, at = c - owner * share;
+                int owner = c / share, at = (c - owner * share) / 4;
 #pragma unroll
                 for (int i = 0; i < CHUNK; i += 4)
                     if (c + i < p.M) {
-                        st_cluster_16(map_to_cta(sums + ((rank * 128 + ch) * share + at) * 4, owner), v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        at += 4;
-                        if (at == share) at = 0, owner++;
+                        st_cluster_16(map_to_cta(sums + ((rank * share + 4 * at) * 32 + ch) * 16, owner), v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        if (4 * ++at == share) at = 0, owner++;
                     }
             });
         __syncwarp();
         cluster_arrive();
         if (own < p.M) {               // (a CTA that finishes no row is written to by none)
             cluster_wait();
-            const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + ch * share;
+            const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + 4 * ch;
             for (int i = 4 * half; i < share && own + i < p.M; i += 8) {
-                float4 s = *reinterpret_cast<const float4*>(mine + i);
+                float4 s = *reinterpret_cast<const float4*>(mine + i * 128);
                 for (uint32_t q = 1; q < split; q++) {
-                    const float4 o = *reinterpret_cast<const float4*>(mine + q * 128 * share + i);
+                    const float4 o = *reinterpret_cast<const float4*>(mine + (q * share + i) * 128);
                     s = make_float4(sum_of(s.x, o.x), sum_of(s.y, o.y), sum_of(s.z, o.z), sum_of(s.w, o.w));
                 }
                 finish4(own + i, s.x, s.y, s.z, s.w);
@@ -288,7 +287,7 @@ cudaError_t launch(FewKernelState& state, int sm_count, const CUtensorMap& map_b
         return fit;
     };
     // The deep ring where all clusters are resident at once with it (1 x 4 096 -> 14 336 12.8 us with two CTAs per SM, 11.7 so).
-    // (of 64 and 128 rows a second round of clusters costs more than a share of K twice as long: 64 x 8 192 -> 2 048 11.2 -> 9.8 us)
+    // (of 64 and 128 rows a second round of clusters costs more than a share of K twice as long: 64 x 8 192 -> 2 048 11.2 us, 9.8 so)
     while (ROWS >= 64 && split > 1 && blocks > resident()) split /= 2;
     const int most = (p.k_blocks + split - 1) / split;
     p.stages = blocks <= resident() ? T::DEEP : T::HALF;

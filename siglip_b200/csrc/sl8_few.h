@@ -8,13 +8,13 @@
 
 namespace sl8 {
 
-// Whether these kernels take a product, rather than tiles of 128 x 64 on single CTAs, which do not share out K: up to 16 rows always; from
-// there on the partial sums that change hands cost 50 - 100 ns a row, which only a deep K pays for.  us here / on such tiles, int8:
-//   16 rows: 768 x 768 2.9 / 3.4, 4 304 x 1 152 3.9 / 4.8, 4 096 x 4 096 6.4 / 10.5, 14 336 x 4 096 12.3 / 26
-//   32: 768 x 768 3.5 / 3.4, 4 304 x 1 152 4.75 / 4.8, 1 152 x 4 304 4.65 / 6.9, 4 096 x 4 096 7.4 / 8.4
-//   64: 4 304 x 1 152 5.3 / 4.4, 1 152 x 4 304 7.0 / 7.1, 4 096 x 4 096 8.7 / 8.6, 14 336 x 4 096 13.2 / 16.6, 4 096 x 14 336 15.3 / 24
-//   128: 4 096 x 4 096 13.9 / 8.8, 4 096 x 8 192 16.8 / 14.9, 4 096 x 14 336 21 / 24.6, 1 024 x 16 384 14.7 / 20.5
-inline bool few_rows(long long M, int K) { return M <= 16 || (M <= 32 && K > 1024) || (M <= 64 && K > 2944) || (M <= 128 && K >= 12288); }
+// Whether these kernels take a product, rather than tiles of 128 x 64 on single CTAs, which do not share out K: the more rows, the
+// deeper K has to be.  us here / on such tiles, int8, by rows:
+//   768 x 768     16: 3.0 / 3.4, 32: 3.2 / 3.4, 64: 4.0 / 3.5           4 304 x 1 152  16: 3.8 / 4.7, 32: 4.1 / 4.7, 64: 5.4 / 4.3
+//   2 048 x 2 048 32: 4.4 / 4.8, 64: 4.7 / 4.8, 128: 6.6 / 5.0          4 096 x 4 096  16: 6.4 / 10.5, 64: 7.5 / 8.5, 128: 9.6 / 8.9
+//   8 192 x 4 096 32: 9.4 / 9.9, 64: 10.4 / 10.1, 128: 12.4 / 10.5      8 192 x 8 192  16: 13.9 / 17.1, 64: 15.5 / 17.6, 128: 17.9 / 18.1
+//   4 096 x 8 192 64: 10.3 / 14.4, 128: 12.4 / 14.9                     4 096 x 14 336 16: 12.9 / 23.6, 64: 14.1 / 24, 128: 16.8 / 24.5
+inline bool few_rows(long long M, int K) { return M <= 32 || (M <= 64 && K >= 2048) || (M <= 128 && K >= 6144); }
 constexpr int kFewSplitMax = 8;            // CTAs of a cluster, each with a share of K
 
 struct FewParams {

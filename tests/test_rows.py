@@ -37,7 +37,7 @@ def row_scales_of(y32: np.ndarray, top: float) -> np.ndarray:
 def row_factors_of(y32: np.ndarray, top: float) -> np.ndarray:
     """What a row's values are multiplied by to become codes: top / max, or the reciprocal of a scale that was too small."""
     amax, scale = np.abs(y32).max(1).astype(np.float32), row_scales_of(y32, top)
-    with np.errstate(divide="ignore"):
+    with np.errstate(divide="ignore", over="ignore"):
         return np.where((amax == 0) | (scale == np.float32(TINY)), np.float32(1) / scale, np.float32(top) / amax).astype(np.float32)
 
 
@@ -362,7 +362,7 @@ def check_linear(got, A, B, sa, sb, bias, gelu, codes):
 
 SHAPES = [(1, 16, 1), (1, 1152, 4304), (2, 48, 16), (3, 128, 31), (8, 144, 128), (15, 272, 129), (16, 4304, 1152), (17, 256, 300), (31, 1168, 588), (32, 64, 2048),
           (33, 400, 1155), (63, 128, 640), (64, 1152, 4304), (65, 1152, 300), (100, 16, 32), (127, 48, 33), (128, 112, 4304), (129, 240, 257), (300, 336, 1155),
-          (65, 144, 12288), (128, 400, 12333), (97, 2048, 12400), (10, 2048, 8192), (50, 2064, 8000), (729, 1152, 588), (257, 4304, 100), (1000, 592, 999)]
+          (65, 144, 6144), (128, 400, 12333), (97, 2048, 6200), (61, 272, 2048), (10, 2048, 8192), (50, 2064, 8000), (729, 1152, 588), (257, 4304, 100), (1000, 592, 999)]
 
 
 @pytest.mark.gpu
