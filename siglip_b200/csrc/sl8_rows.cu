@@ -302,6 +302,129 @@ __global__ void __launch_bounds__(WARP ? kWarpRowThreads : CH == 1 ? 1024 : 512)
     }
 }
 
+// Rows of up to 256 elements (heads, groups), many: LANES lanes to a row, eight elements a lane; its gamma stays in registers.  Bound by the
+// bytes, and by what a row costs besides them (its reductions and divisions): bf16 -> int8 500 000 x 64 23 us (a warp to a row, ring 81), x 128
+// 44 (81); norm with a residual 47 (167) and 89 (167), two rows of a lane at a time (one 53 and 104, four 50 and 94; without the
+// norm one 23, two 25, four 27).  200 000 x 100 bf16, element by element, 29 (53).
+constexpr int kNarrowThreads = 256;
+__host__ __device__ constexpr int narrow_rows(bool norm, bool vec) { return norm && vec ? 2 : 1; }      // of a lane at a time
+template <typename T, bool NORM, bool VEC, int LANES>
+__global__ void __launch_bounds__(kNarrowThreads, !NORM && VEC ? 6 : NORM && sizeof(T) == 4 ? 3 : 4) narrow_row_kernel(const RowArgs a) {
+    constexpr int U = narrow_rows(NORM, VEC), PER_WARP = 32 / LANES, STEP = VEC ? 1 : LANES;
+    const int lane = threadIdx.x & 31, l = lane % LANES, c0 = VEC ? 8 * l : l;
+    const int left = a.cols - c0;                                            // elements from this lane's first on
+    sl8::pdl_wait();
+    sl8::pdl_release();
+    const float given = a.scale ? sl8::ld_f32(a.scale) : 1.0f;
+    float g[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) g[i] = NORM && a.gamma && STEP * i < left ? sl8::ld_f32(a.gamma + c0 + STEP * i) : 1.0f;
+    const long long warps = static_cast<long long>(gridDim.x) * (kNarrowThreads / 32);
+    for (long long base = (blockIdx.x * static_cast<long long>(kNarrowThreads / 32) + (threadIdx.x >> 5)) * (PER_WARP * U); base < a.rows; base += warps * (PER_WARP * U)) {
+        const long long first = base + lane / LANES;                         // this lane's rows: first, first + PER_WARP, ...
+        const auto live = [&](int u) { return left > 0 && first + u * PER_WARP < a.rows; };
+        const auto row = [&](const void* p, long long ld, int u) { return static_cast<const T*>(p) + (first + u * PER_WARP) * ld + c0; };
+        const auto take = [&](Eight<T>& e, const T* p) {
+            if constexpr (VEC) {
+                fetch<true>(e, p, left);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const T* const at = p + STEP * min(i, (left - 1) / STEP);         // (the last one in the place of those beyond)
+                    uint32_t b;
+                    if constexpr (sizeof(T) == 4) b = __float_as_uint(sl8::ld_f32(at));
+                    else b = ld_u16(at);
+                    if (STEP * i >= left) b = 0u;
+                    if constexpr (sizeof(T) == 4) e.w[i] = b;
+                    else if (i & 1) e.w[i / 2] |= b << 16;
+                    else e.w[i / 2] = b;
+                }
+            }
+        };
+        Eight<T> e[U], f[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (live(u)) take(e[u], row(a.x, a.ld, u));
+        if (NORM && a.residual) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (live(u)) take(f[u], row(a.residual, a.ld_res, u));
+        }
+        float v[U][8];
+        Stats s[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            s[u] = Stats{0.0f, 0.0f};
+            if (!live(u)) continue;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[u][i] = value(e[u], i);
+            if constexpr (NORM) {
+                if (a.residual) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[u][i] += value(f[u], i);
+                    T* const sum = static_cast<T*>(a.sum) + (first + u * PER_WARP) * a.ld_sum + c0;
+                    if constexpr (VEC) {
+                        put_sum<true>(sum, v[u], left);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (STEP * i < left) {
+                                if constexpr (sizeof(T) == 4) sum[STEP * i] = v[u][i];
+                                else sum[STEP * i] = __float2bfloat16_rn(v[u][i]);
+                            }
+                    }
+                }
+                float odd = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    s[u].squares = fmaf(v[u][i], v[u][i], s[u].squares);
+                    odd = fmaf(v[u][i + 1], v[u][i + 1], odd);
+                }
+                s[u].squares += odd;
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[u][i] *= g[i];
+            }
+            s[u].largest = largest_of(0.0f, v[u]);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if constexpr (NORM) s[u].squares += __shfl_xor_sync(0xffffffffu, s[u].squares, o);
+                s[u].largest = __uint_as_float(max(__float_as_uint(s[u].largest), __shfl_xor_sync(0xffffffffu, __float_as_uint(s[u].largest), o)));
+            }
+        // every lane knows the sums of its rows: of two rows, one lane in two works out one of them, and the others ask it
+        Stats one = s[0];
+        if (U == 2 && (l & 1)) one = s[U - 1];
+        const Scaling of_one = scaling<NORM>(a, one, given);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            Scaling k = of_one;
+            if constexpr (U == 2) {
+                const int from = lane / LANES * LANES + u;
+                k.k = __shfl_sync(0xffffffffu, of_one.k, from);
+                k.scale = __shfl_sync(0xffffffffu, of_one.scale, from);
+                k.rstd = __shfl_sync(0xffffffffu, of_one.rstd, from);
+                k.small = __shfl_sync(0xffffffffu, static_cast<int>(of_one.small), from) != 0;
+            }
+            if (!live(u)) continue;
+            if (k.small) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[u][i] *= k.rstd;
+            }
+            uint8_t* const out = a.out + (first + u * PER_WARP) * a.ld_out + c0;
+            if constexpr (VEC) {
+                put_codes<true>(out, v[u], k.k, a.int8 != 0, left);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (STEP * i < left) out[STEP * i] = static_cast<uint8_t>(a.int8 ? int8_of(v[u][i], k.k) : sl8::pack_e4m3x2(v[u][i] * k.k, 0.0f));
+            }
+            if (a.row_scales && l == 0) a.row_scales[first + u * PER_WARP] = k.scale;
+        }
+    }
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
@@ -591,25 +714,32 @@ cudaError_t stream_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     return sl8_launch_chained(kernel, static_cast<unsigned>(want < once * waves ? want : once * waves), threads, bytes, s, a, span);
 }
 
+template <typename T, bool NORM, bool VEC, int LANES>
+cudaError_t narrow(int sm_count, cudaStream_t s, const RowArgs& a) {
+    constexpr int ROWS = kNarrowThreads / LANES * narrow_rows(NORM, VEC);
+    const long long want = (a.rows + ROWS - 1) / ROWS, cap = static_cast<long long>(sm_count) * 16;
+    return sl8_launch_chained(narrow_row_kernel<T, NORM, VEC, LANES>, static_cast<unsigned>(want < cap ? want : cap), kNarrowThreads, 0, s, a);
+}
+
 // Up to ten rows per SM: a block each, one trip to memory (1 500 x 4 304 bf16 -> int8 5.9 us, ring 6.5); with all eight elements of a
 // thread's at once while 256 threads do (norm of one row of 1 152 1.74 us, 1.95 with three times eight), with three from there on (729 x 4 304
-// 3.6 us, 5.4 with one).  Up to forty, where rows are short: a warp each (norm of 5 003 x 1 152 10.3 us, ring 10.9).  Then the ring, by
+// 3.6 us, 5.4 with one).  Of up to 256 elements: several to a warp.  Up to forty rows per SM, where they are short: a warp each (norm of 5 003 x 1 152 10.3 us, ring 10.9).  Then the ring, by
 // warps while rows are short, by blocks of three times eight elements a thread (100 000 x 512 57 us by warps, 64 by blocks; 20 000 x
 // 2 048 50 either way; 46 656 x 4 304 92, 94 with four, 96 with two), and rows on odd addresses from the tenth row per SM (norm of
 // 5 003 x 1 155 15.5 us, in registers 30).
 template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     const bool few = a.rows <= 10ll * sm_count;
-    if (few || a.cols * sizeof(T) < 16) {
+    if (!few && a.cols <= 256) return a.cols <= 64 ? narrow<T, NORM, VEC, 8>(sm_count, s, a) : a.cols <= 128 ? narrow<T, NORM, VEC, 16>(sm_count, s, a) : narrow<T, NORM, VEC, 32>(sm_count, s, a);
+    if (few) {
         if (a.cols <= 2048) return direct<T, NORM, VEC, 1, false>(sm_count, s, a);
         if (a.cols <= 12288) return direct<T, NORM, VEC, 3, false>(sm_count, s, a);
     }
     if constexpr (VEC) {
         if (a.rows <= 40ll * sm_count && a.cols <= 1280)
-            return a.cols <= 256 ? direct<T, NORM, true, 1, true>(sm_count, s, a) : a.cols <= 768 ? direct<T, NORM, true, 3, true>(sm_count, s, a) : direct<T, NORM, true, 5, true>(sm_count, s, a);
+            return a.cols <= 768 ? direct<T, NORM, true, 3, true>(sm_count, s, a) : direct<T, NORM, true, 5, true>(sm_count, s, a);
         if (a.cols > 768 && a.cols <= 1280) return stream_rows<T, NORM, true, 5, true>(sm_count, s, a);
     }
-    if (a.cols <= 256) return stream_rows<T, NORM, VEC, 1, true>(sm_count, s, a);
     if (a.cols <= 512) return stream_rows<T, NORM, VEC, 2, true>(sm_count, s, a);
     if (a.cols <= 768) return stream_rows<T, NORM, VEC, 3, true>(sm_count, s, a);
     if constexpr (!VEC)

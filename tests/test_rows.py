@@ -235,7 +235,8 @@ def test_rmsnorm_pitched_operands(engine):
 
 # ----------------------------------------------------------------------------- many rows: rings in shared memory, several rows per warp or block
 # (rows, columns, elements ahead of the first row, pitch): whole vectors and not, each width that has a kernel of its own
-MANY = [(6100, 8, 0, 8), (6001, 256, 8, 272), (6011, 504, 0, 512), (6003, 768, 0, 768), (6007, 1152, 16, 1160), (12345, 1280, 0, 1280), (1481, 1288, 8, 1296), (2999, 2048, 0, 2048),
+MANY = [(6100, 8, 0, 8), (9001, 64, 0, 64), (20003, 72, 0, 1152), (7001, 128, 8, 144), (5999, 120, 0, 128), (1481, 40, 0, 40), (300001, 16, 0, 16),
+        (5003, 1, 0, 1), (3001, 1, 5, 3), (4001, 4, 0, 4), (9003, 7, 1, 7), (8001, 63, 0, 63), (7777, 65, 0, 65), (6666, 100, 0, 100), (2222, 129, 1, 130), (3333, 200, 4, 201), (6001, 256, 8, 272), (6011, 504, 0, 512), (6003, 768, 0, 768), (6007, 1152, 16, 1160), (12345, 1280, 0, 1280), (1481, 1288, 8, 1296), (2999, 2048, 0, 2048),
         (1777, 4304, 0, 4304), (1483, 8192, 0, 8192), (1482, 12288, 0, 12288), (1490, 12296, 8, 12304), (1485, 16384, 0, 16384), (1481, 16392, 0, 16392),
         (1700, 9, 1, 9), (1600, 13, 0, 17), (1503, 255, 3, 255), (1502, 256, 1, 257), (2001, 333, 0, 333), (1600, 511, 5, 600), (1555, 767, 0, 768), (1500, 769, 7, 769),
         (3001, 1155, 0, 1155), (1490, 2047, 1, 2049), (1481, 2050, 0, 2050), (1482, 4305, 3, 4305), (1483, 12287, 0, 12287), (1484, 12290, 1, 12290), (1481, 16383, 0, 16383),
@@ -305,6 +306,7 @@ def test_rmsnorm_of_many_rows(engine, dtype, rows, cols, ahead, pitch):
                 y = y.clamp(-448 * 0.02, 448 * 0.02)
             else:
                 want = y.abs().amax(1, keepdim=True) / TOP[codes]
+                want = torch.where(want == 0, 1.0, want)         # (a row of zeros: of one column, x = -residual)
                 assert ((s - want).abs() <= want * (rel + 2.0 ** -23)).all()
             half = (s / 2).expand_as(y) if kind == I8 else torch.maximum(y.abs() * (1 + 2 * rel) * 2.0 ** -4, s * 2.0 ** -10)
             value = (q[part] if kind == I8 else q[part].view(F8)).double() * s
