@@ -3,9 +3,9 @@
 // What takes time is the weights' way in, so the product is turned round: 128 rows of B are the M of a tcgen05.mma, the rows of A (16,
 // 32, 64 or 128, what is missing read as zeros) its N, and a CTA brings 16 KiB of weights per k-block for 2 - 16 KiB of
 // activations.  K is shared out to the CTAs of a cluster, because the weights of few output channels would otherwise come through few
-// SMs (1 x 4 304 -> 1 152: 8 CTAs 3.8 us, 4 4.4, 2 6.0).  Each CTA writes its partial sums into the shared memory of the one that
+// SMs (1 x 4 304 -> 1 152: 8 CTAs 4.0 us, 4 4.4, 2 6.0).  Each CTA writes its partial sums into the shared memory of the one that
 // finishes the row, four rows at a time, and one cluster barrier stands between that and the adding up: exact for int8, in the order of
-// the ranks for e4m3, so the same result every time.  (Read from there instead, with a barrier on either side: 4.4 us.)
+// the ranks for e4m3, so the same result every time.  (Read from there instead, with a barrier on either side: 4.6 us.)
 // Bound by the weights' bytes where there are many (32 768 x 4 096, 134 MB: 22.4 us, 6.0 TB/s; 8 192 x 8 192 13.3 us, 5.0), by the way
 // of one k-block through all of it where there are few: about 2.8 us from launch to launch (768 x 768).
 #include "sl8_kernel.cuh"
@@ -67,6 +67,11 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     wc.peer_abort = 0u;              // (the other CTAs of the cluster wait for nothing but its barriers, which every CTA reaches)
     wc.tile = blockIdx.x / split;
 
+    // No CTA waits for another one of its cluster while it holds tensor memory: that one may itself be waiting for tensor memory, behind a
+    // kernel of another stream whose CTAs wait for one another as well (a pair's of the GEMM), and they for what this one holds.  So a CTA says
+    // that it runs ahead of the allocation (what another has to know before it writes to its shared memory), and gives the tensor memory
+    // back before it waits for the second time.
+    if (split > 1) cluster_arrive();
     if (warp == 0) {
         if (lane < 2 * p.stages + 1) {
             mbar_init(full0 + 8 * lane, 1);
@@ -89,7 +94,6 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
-    if (split > 1) cluster_arrive();         // (every CTA of the cluster runs before one writes to another's shared memory)
     pdl_wait();
     pdl_release();       // (behind the allocation of tensor memory, on which no later kernel may be ahead of this one)
 
@@ -186,6 +190,21 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
             f(c, v);
         }
     };
+    const auto release = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        if (*abort_flag) {         // copies and MMAs in flight land before their memory is released
+            const unsigned long long t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 200000ull) {
+            }
+            __syncthreads();
+        }
+        if (warp == 1) {
+            tc_fence_after();
+            tmem_dealloc<1>(tmem, T::TMEM_COLS);
+        }
+        __syncwarp();
+    };
     if (split == 1) {
         if (ok)
             chunks([&](int c, const float* v) {
@@ -193,6 +212,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
                 for (int i = 0; i < CHUNK; i += 4)
                     if (c + i < p.M) finish4(c + i, v[i], v[i + 1], v[i + 2], v[i + 3]);
             });
+        release();
     } else {
         // Each rank of the cluster finishes `share` rows, a multiple of four: it gets their sums from every rank.
         const int share = p.share, own = static_cast<int>(rank) * share;
@@ -209,6 +229,7 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
             });
         __syncwarp();
         cluster_arrive();
+        release();                     // (while the others arrive)
         if (own < p.M) {               // (a CTA that finishes no row is written to by none)
             cluster_wait();
             const float* const mine = reinterpret_cast<const float*>(few_smem + (sums - raw)) + 4 * ch;
@@ -221,19 +242,6 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const __grid_cons
                 finish4(own + i, s.x, s.y, s.z, s.w);
             }
         }
-    }
-
-    tc_fence_before();
-    __syncthreads();
-    if (*abort_flag) {         // copies and MMAs in flight land before their memory is released
-        const unsigned long long t0 = globaltimer_ns();
-        while (globaltimer_ns() - t0 < 200000ull) {
-        }
-        __syncthreads();
-    }
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc<1>(tmem, T::TMEM_COLS);
     }
 }
 

@@ -602,6 +602,33 @@ def test_two_streams_at_once(engine):
 
 
 @pytest.mark.gpu
+def test_clusters_beside_pairs_on_another_stream():
+    """The kernels for few rows share SMs with those of CTA pairs that leave them room: neither waits for its partners while it holds
+    what the other's partners wait for (tensor memory)."""
+    from siglip_b200 import Engine
+    with Engine(0) as pairs, Engine(0) as few:
+        pairs.set_variant(13)                     # the least shared memory of the pairs
+        A, _ = operand(3000, 1152, F8, 1)
+        W, _ = operand(1024, 1152, F8, 2)
+        x, sx = operand(5, 1152, I8, 3)
+        w, sw = operand(1152, 1152, I8, 4)
+        one = torch.tensor([0.01], device=DEV)
+        want_a, want_b = pairs.linear_bias(A, W, None, scale_a=one), few.linear_scaled(x, w, sx, sw)
+        torch.cuda.synchronize()
+        got_a, got_b = torch.empty_like(want_a), torch.empty_like(want_b)
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        for _ in range(100):
+            pairs.linear_bias(A, W, None, scale_a=one, out=got_a, stream=streams[0])
+            for st in streams[1:]:
+                for _ in range(4):
+                    few.linear_scaled(x, w, sx, sw, out=got_b, stream=st)
+        torch.cuda.synchronize()
+        pairs.device_status()
+        few.device_status()
+        assert torch.equal(got_a, want_a) and torch.equal(got_b, want_b)
+
+
+@pytest.mark.gpu
 def test_static_norm_feeds_the_layers_that_were_there(engine):
     x, r = activations(197, 768, BF16, 1), activations(197, 768, BF16, 2)
     scale = torch.tensor([8.0 / 448.0], device=DEV)
