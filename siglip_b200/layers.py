@@ -473,10 +473,10 @@ class Engine:
         """`out`, or new codes of `dtype` on rows of 128-byte lines."""
         if dtype not in self._ROW_TYPES:
             raise TypeError("codes with a scale for each row are int8, float8_e4m3fn or uint8 (raw e4m3 codes)")
+        self._on_device("x", x)           # (some of these kernels copy rows in bulk: pinned host memory is not for them)
         if out is None:
-            self._on_device("x", x)
             return torch.empty((rows, (cols + 127) // 128 * 128), dtype=torch.uint8, device=x.device).view(dtype)[:, :cols]
-        self._readable("x", x)
+        self._on_device("out", out)
         self._codes_into(out, rows, cols, (torch.int8,) if dtype == torch.int8 else self._E4M3_TYPES)
         if _code_type(out.dtype) != _code_type(dtype):        # (a pitch that the library refuses is not looked at above)
             raise TypeError(f"dtype {dtype} contradicts out.dtype {out.dtype}")
@@ -487,7 +487,7 @@ class Engine:
         if scales is None:
             return torch.empty((rows,), dtype=torch.float32, device=device)
         self._floats("scales", scales, rows)
-        self._readable("scales", scales)
+        self._on_device("scales", scales)
         return scales
 
     def _stream_of(self, x, residual, summed, rows: int, cols: int):
@@ -501,9 +501,8 @@ class Engine:
                 continue
             if t.dtype != x.dtype or tuple(t.shape) != (rows, cols) or (t.stride(1) != 1 and cols != 1):
                 raise ValueError(f"{name} must be {x.dtype} [{rows}, {cols}] with the columns contiguous, like x")
-            self._readable(name, t)
+            self._on_device(name, t)
         if summed is None:
-            self._on_device("x", x)
             summed = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
         return summed
 
@@ -536,7 +535,7 @@ class Engine:
                 return self._done(r)
         rows, cols = self._rows(x)
         self._floats("gamma", gamma, cols)
-        self._readable("gamma", gamma)
+        self._on_device("gamma", gamma)
         out = self._row_codes(x, rows, cols, dtype, out)
         scales = self._row_scales(scales, rows, out.device)
         return self._rmsnorm(x, rows, cols, gamma, eps, residual, summed, None, out, scales, stream)
@@ -551,7 +550,7 @@ class Engine:
         rows, cols = self._rows(x)
         for name, t, n in (("gamma", gamma, cols), ("scale", scale, 1)):
             self._floats(name, t, n)
-            self._readable(name, t)
+            self._on_device(name, t)
         out = self._row_codes(x, rows, cols, torch.uint8, out)
         return self._rmsnorm(x, rows, cols, gamma, eps, residual, summed, scale, out, None, stream)
 

@@ -684,6 +684,17 @@ def test_a_row_that_never_comes(monkeypatch, cols):
 
 
 @pytest.mark.gpu
+def test_pinned_memory_is_refused(engine):
+    x, host = activations(8, 64, BF16, 1), torch.zeros((8, 64), dtype=BF16).pin_memory()
+    for call in (lambda: engine.quantize_rows(host), lambda: engine.quantize_rows(x, out=torch.zeros((8, 64), dtype=I8).pin_memory()),
+                 lambda: engine.quantize_rows(x, scales=torch.zeros(8).pin_memory()), lambda: engine.rmsnorm_quantize_rows(host),
+                 lambda: engine.rmsnorm_quantize_rows(x, torch.zeros(64).pin_memory()), lambda: engine.rmsnorm_quantize_rows(x, residual=host),
+                 lambda: engine.rmsnorm_quantize_rows(x, residual=x, summed=host.clone().pin_memory()), lambda: engine.rmsnorm_quantize(x, scale=torch.ones(1).pin_memory())):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.gpu
 def test_the_library_refuses(engine):
     """Straight at the C ABI: what the Python checks would stop."""
     lib, h = engine._lib, engine._h
