@@ -666,8 +666,8 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const RowArgs a)
 // ---- which kernel, on how many blocks
 constexpr size_t kRingBytes = 227 * 1024 - 1024;       // shared memory of a block, less what the kernel declares itself
 template <typename Kernel>
-cudaError_t allow_shared(Kernel kernel, size_t bytes) {
-    return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+cudaError_t allow_shared(Kernel kernel, size_t bytes) {          // (48 KiB need no leave, what the kernel declares itself included)
+    return bytes > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
 }
 
 template <typename T, bool NORM, bool VEC>

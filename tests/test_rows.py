@@ -146,7 +146,7 @@ def norm_error(cols):
 @pytest.mark.parametrize("codes", [I8, F8, "static"])
 @pytest.mark.parametrize("residual,gamma", [(True, True), (False, True), (True, False), (False, False)])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 13), (1, 1152), (65, 768), (1001, 1152), (5, 1157), (4, 2048), (3, 2056), (130, 4304), (2, 8192), (3, 16384),
-                                       (2, 17000), (1, 33001)])
+                                       (2, 12288), (3, 12192), (7, 12160), (2, 10300), (2, 17000), (1, 33001)])
 def test_rmsnorm_against_64_bits(engine, dtype, codes, residual, gamma, rows, cols):
     x = activations(rows, cols, dtype, cols + rows)
     r = activations(rows, cols, dtype, cols + rows + 1, std=3.0) if residual else None
