@@ -665,9 +665,12 @@ __global__ void __launch_bounds__(kLongThreads) long_row_kernel(const RowArgs a)
 
 // ---- which kernel, on how many blocks
 constexpr size_t kRingBytes = 227 * 1024 - 1024;       // shared memory of a block, less what the kernel declares itself
+constexpr size_t kDirectBytes = 12288 * sizeof(float); // gamma of the widest rows of row_kernel
+// Leave to launch with `bytes` of shared memory (48 KiB need none, what the kernel declares itself included).  It belongs to the kernel on the
+// device, which every thread and handle shares: each asks for the same, the most that any call can need, so none takes another's away.
 template <typename Kernel>
-cudaError_t allow_shared(Kernel kernel, size_t bytes) {          // (48 KiB need no leave, what the kernel declares itself included)
-    return bytes > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) : cudaSuccess;
+cudaError_t allow_shared(Kernel kernel, size_t bytes, size_t most) {
+    return bytes > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)) : cudaSuccess;
 }
 
 template <typename T, bool NORM, bool VEC>
@@ -680,7 +683,7 @@ template <typename T, bool NORM, bool VEC, int CH, bool WARP>
 cudaError_t direct(int sm_count, cudaStream_t s, const RowArgs& a) {
     const auto kernel = row_kernel<T, NORM, VEC, CH, WARP>;
     const size_t bytes = NORM && a.gamma ? sizeof(float) * a.cols : 0;
-    const cudaError_t e = allow_shared(kernel, bytes);
+    const cudaError_t e = allow_shared(kernel, bytes, kDirectBytes);
     if (e != cudaSuccess) return e;
     constexpr int ROWS = WARP ? kWarpRowThreads / 32 : 1;
     const int threads = WARP ? kWarpRowThreads : ((a.cols + 7) / 8 + CH * 32 - 1) / (CH * 32) * 32;
@@ -699,7 +702,7 @@ cudaError_t stream_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     const int span = (a.cols * static_cast<int>(sizeof(T)) + 16 + 127) / 128 * 128;
     const size_t bytes = gamma_bytes(NORM && a.gamma, a.cols) + static_cast<size_t>(GROUPS) * kSlots * span * (a.residual ? 2 : 1);
     if (bytes > kRingBytes) return launch_long<T, NORM, VEC>(sm_count, s, a);
-    const cudaError_t e = allow_shared(kernel, bytes);
+    const cudaError_t e = allow_shared(kernel, bytes, kRingBytes);
     if (e != cudaSuccess) return e;
     const int threads = WARP ? kWarpRowThreads : ((a.cols + 7) / 8 + CH * 32 - 1) / (CH * 32) * 32;
     // Blocks that are resident at once, and from some rows per block on several times as many: the SMs do not get through their rows
