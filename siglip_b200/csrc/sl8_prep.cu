@@ -226,7 +226,9 @@ template <typename PT, int MODE, bool ALIGNED, int BATCH>
 cudaError_t launch_unfold_batch(unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const PT* pixels, long long total, int H, int W, int P, int C, int gh, int gw,
                                 int G, int groups, int rows_per_step, int chunks, const float* scale, uint8_t* A, long long lda, int row_bytes) {
     if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(patchify_quantize_kernel<PT, MODE, ALIGNED, BATCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // the most that a block can have, not what this call needs: the limit belongs to the kernel on the device, and a thread with smaller patches
+        // must not lower it between here and the launch
+        const cudaError_t e = cudaFuncSetAttribute(patchify_quantize_kernel<PT, MODE, ALIGNED, BATCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         if (e != cudaSuccess) return e;
     }
     return sl8_launch_chained(patchify_quantize_kernel<PT, MODE, ALIGNED, BATCH>, grid, threads, smem, s, pixels, total, H, W, P, C, gh, gw, G, groups, rows_per_step,

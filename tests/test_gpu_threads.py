@@ -55,3 +55,25 @@ def test_row_kernels_of_different_widths(handles, rows, widths):
         e.close()
     for got, want, *_ in checks:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_patch_unfolds_of_different_sizes():
+    """The same of the patch unfold: patches of 64 x 64 and of 128 x 128 take 48 and 96 KiB in one kernel."""
+    e = Engine(0)
+    calls, checks, streams = [], [], [torch.cuda.Stream() for _ in range(4)]
+    scale = torch.tensor([0.02], device=DEV)
+    for i, stream in enumerate(streams):
+        channels, patch = ((6, 64), (3, 128))[i % 2]
+        pixels = torch.randn((8, channels, patch, patch), generator=torch.Generator(device=DEV).manual_seed(i), device=DEV).to(BF16)
+        want = e.patchify_quantize(pixels, patch, scale)
+        out = torch.zeros_like(want)
+        args = (e._h, pixels.data_ptr(), L.SL8_DT_BF16, 8, channels, patch, patch, patch, scale.data_ptr(), out.data_ptr(), out.stride(0), C.c_void_p(stream.cuda_stream))
+        calls.append(lambda args=args: e._lib.sl8_patchify_quantize_e4m3(*args))
+        checks.append((out, want, pixels))
+    torch.cuda.synchronize()
+    assert from_threads(calls, 1500) == [{L.SL8_OK}] * len(calls)
+    torch.cuda.synchronize()
+    e.close()
+    for out, want, _ in checks:
+        assert torch.equal(out, want)
