@@ -112,8 +112,8 @@ typedef struct sl8_config {
 int sl8_create(sl8_handle_t* h, int device);
 int sl8_destroy(sl8_handle_t h);
 
-/* Text of the last failure on this handle (never NULL).  With h == NULL: the last
- * failure of sl8_create on the calling thread. */
+/* Text of the last failure on this handle, whichever thread's (never NULL).  With h == NULL: the last
+ * failure of sl8_create on the calling thread.  The text is the calling thread's and stays until it asks for this handle's again. */
 const char* sl8_last_error_string(sl8_handle_t h);
 
 /* Library identification: "siglip_fp8 <version> sm_100a". */

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <map>
 
 #include "sl8_internal.h"
 #include "sl8_dispatch_table.h"
@@ -38,8 +39,12 @@ thread_local std::string g_create_error;
 }  // namespace
 
 int sl8_fail(sl8_handle_t h, int code, const std::string& msg) {
-    if (h) h->err = msg;
-    else g_create_error = msg;
+    if (h) {
+        std::lock_guard<std::mutex> lock(h->err_mu);
+        h->err = msg;
+    } else {
+        g_create_error = msg;
+    }
     return code;
 }
 
@@ -502,7 +507,12 @@ SL8_API int sl8_destroy(sl8_handle_t h) {
 
 SL8_API const char* sl8_last_error_string(sl8_handle_t h) {
     if (!h) return g_create_error.c_str();
-    return h->err.c_str();
+    // the calling thread's copy: another one may fail, and write the handle's text, while this one reads
+    thread_local std::map<sl8_handle_t, std::string> copies;
+    std::string& copy = copies[h];
+    std::lock_guard<std::mutex> lock(h->err_mu);
+    copy = h->err;
+    return copy.c_str();
 }
 
 // =========================================================================== layers

@@ -69,8 +69,9 @@ struct sl8_context {
     bool smem_attr_set[SL8_NUM_VARIANTS][sl8::K_COUNT] = {};
     int max_clusters[SL8_NUM_VARIANTS][sl8::K_COUNT] = {};
     sl8::FewState few;
-    std::mutex mu;          // the handle's state during one launch (map cache, attributes, error text)
+    std::mutex mu;          // the handle's state during one launch (map cache, attributes)
     std::mutex pipe_mu;     // the host-operand pipeline during one *_host call (taken before mu)
+    std::mutex err_mu;      // err: calls of several threads may fail at once, most of them before they take mu
     std::string err;
     Sl8HostPipe pipe;
 };

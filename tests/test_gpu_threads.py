@@ -77,3 +77,20 @@ def test_patch_unfolds_of_different_sizes():
     e.close()
     for out, want, _ in checks:
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_texts_of_calls_that_fail_at_once():
+    """Refused calls of several threads on one handle: each text that is read is one that was written."""
+    with Engine(0) as e:
+        x, out, scales = torch.zeros((4, 64), dtype=BF16, device=DEV), torch.zeros((4, 64), dtype=I8, device=DEV), torch.zeros((4,), device=DEV)
+
+        def refused(dtype, code_type, at):
+            assert e._lib.sl8_quantize_rows(e._h, x.data_ptr() + at, dtype, 4, 64, 64, code_type, out.data_ptr(), 64, scales.data_ptr(), None) != L.SL8_OK
+            return e._lib.sl8_last_error_string(e._h)
+
+        calls = [lambda: refused(7, 1, 0), lambda: refused(1, 9, 0), lambda: refused(1, 1, 1)]
+        texts = {call() for call in calls}
+        assert len(texts) == 3 and all(texts)
+        for got in from_threads(calls * 3, 20000):
+            assert got <= texts
