@@ -235,7 +235,9 @@ int sl8_layernorm_quantize_e4m3(sl8_handle_t h, const void* x, int dtype, int64_
 enum { SL8_CODE_E4M3 = 0, SL8_CODE_INT8 = 1 };
 
 /* row_scales[r] = max |x[r, :]| / 127 (int8) or / 448 (e4m3), 1 for a row of zeros, never below 2^-126;
- * out[r, c] = round(x[r, c] * (127 or 448 / max |x[r, :]|)), ties to even: an activation, or weights [N, K].  A row with an infinity or a
+ * out[r, c] = round(x[r, c] * (127 or 448 / max |x[r, :]|)), ties to even: an activation, or weights [N, K].  Of bf16 rows the quotient is rounded as
+ * if it were exact; of fp32 rows 127 or 448 / max is rounded to fp32 first, so that a quotient within 2^-23 of a tie may go to either side of it.  (Where the
+ * scale is 2^-126, out = round(x / scale).)  A row with an infinity or a
  * NaN gets the scale NaN (and no meaningful codes), so that whatever is computed from it is NaN, and no other row is touched.
  * x fp32 or bf16, any number of columns up to 2^30; x and out are device memory (pinned host memory, which the producer-side steps
  * above read in place, is not for this one and the next); fastest where cols is a multiple of 8 and the rows of x start on 16-byte, those of out on
