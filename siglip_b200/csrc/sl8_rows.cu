@@ -583,7 +583,8 @@ __global__ void __launch_bounds__(WARP ? kWarpRowThreads : 512) row_stream_kerne
             ok = sl8::wait_bar<true>(bar0 + 8 * s, (phases >> s) & 1u, wc, sl8::ST_ROW_WAIT, s);
             phases ^= 1u << s;
         }
-        if (WARP && !__all_sync(0xffffffffu, ok)) break;
+        // a row that has not come is not touched (its sum may go where x or the residual is): all of its threads know before the first writes
+        if (WARP ? !__all_sync(0xffffffffu, ok) : residual && !__syncthreads_and(ok)) break;
         float v[CH][8];
         Stats st = {0.0f, 0.0f};
         float squares[4] = {0.0f, 0.0f, 0.0f, 0.0f};
