@@ -239,9 +239,9 @@ enum { SL8_CODE_E4M3 = 0, SL8_CODE_INT8 = 1 };
  * if it were exact; of fp32 rows 127 or 448 / max is rounded to fp32 first, so that a quotient within 2^-23 of a tie may go to either side of it.  (Where the
  * scale is 2^-126, out = round(x / scale).)  A row with an infinity or a
  * NaN gets the scale NaN (and no meaningful codes), so that whatever is computed from it is NaN, and no other row is touched.
- * x fp32 or bf16, any number of columns up to 2^30; x and out are device memory (pinned host memory, which the producer-side steps
- * above read in place, is not for this one and the next); fastest where cols is a multiple of 8 and the rows of x start on 16-byte, those of out on
- * 8-byte boundaries. */
+ * x fp32 or bf16, any number of columns up to 2^30; all operands are device memory (pinned host memory, which the producer-side steps above read in
+ * place, is not for this call and the next: x or residual there is SL8_ERR_INVALID_VALUE where rows are copied in bulk, from ten rows per SM on).  Fastest
+ * where cols is a multiple of 8 and the rows of x start on 16-byte, those of out on 8-byte boundaries. */
 int sl8_quantize_rows(sl8_handle_t h, const void* x, int dtype, int64_t rows, int cols, int64_t ld, int code_type,
                       void* out, int64_t ld_out, float* row_scales, sl8_stream_t stream);
 

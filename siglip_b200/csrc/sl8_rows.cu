@@ -769,9 +769,10 @@ cudaError_t narrow(int sm_count, cudaStream_t s, const RowArgs& a) {
 // warps while rows are short, by blocks of three times eight elements a thread (100 000 x 512 57 us by warps, 64 by blocks; 20 000 x
 // 2 048 50 either way; 46 656 x 4 304 92, 94 with four, 96 with two), and rows on odd addresses from the tenth row per SM (norm of
 // 5 003 x 1 155 15.5 us, in registers 30).
+bool few_rows(int sm_count, const RowArgs& a) { return a.rows <= 10ll * sm_count; }
 template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
-    const bool few = a.rows <= 10ll * sm_count;
+    const bool few = few_rows(sm_count, a);
     if (!few && a.cols <= 256) return a.cols <= 64 ? narrow<T, NORM, VEC, 8>(sm_count, s, a) : a.cols <= 128 ? narrow<T, NORM, VEC, 16>(sm_count, s, a) : narrow<T, NORM, VEC, 32>(sm_count, s, a);
     if (few) {
         if (a.cols <= 2048) return direct<T, NORM, VEC, 1, false>(sm_count, s, a);
@@ -791,10 +792,22 @@ cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     return launch_long<T, NORM, VEC>(sm_count, s, a);
 }
 
+// The kernels with a ring take rows by bulk copies, which are for memory of a GPU (asked only where one may be taken: 0.1 us on the host).
+bool on_the_host(const void* p) {
+    cudaPointerAttributes at = {};
+    if (!p || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return false;
+    }
+    return at.type == cudaMemoryTypeHost || at.type == cudaMemoryTypeUnregistered;
+}
+
 template <typename T, bool NORM>
 int run_rows(sl8_handle_t h, const RowArgs& a, sl8_stream_t stream, const char* what) {
     Sl8DeviceGuard guard(h->device);
     if (!guard.ok) return sl8_fail(h, SL8_ERR_CUDA, "cudaSetDevice failed");
+    if (!few_rows(h->sm_count, a) && a.cols > 256 && (on_the_host(a.x) || on_the_host(a.residual)))
+        return sl8_fail(h, SL8_ERR_INVALID_VALUE, "x and residual must be device memory: host memory is not copied in bulk");
     constexpr int PER_16 = 16 / sizeof(T);
     // eight elements per access where every row allows it, element by element otherwise
     const bool vec = a.cols % 8 == 0 && sl8_aligned16(a.x) && a.ld % PER_16 == 0 && a.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7u) == 0 &&
