@@ -251,7 +251,8 @@ int sl8_quantize_rows(sl8_handle_t h, const void* x, int dtype, int64_t rows, in
  * are fp32.  With a residual, sum receives h (rounded once to `dtype`): the new residual stream.  sum may be x or the residual itself
  * (same address and leading dimension), but not overlap them otherwise.  gamma fp32 [cols] (NULL = 1).
  *   row_scales given: codes and a scale for each row of y, as sl8_quantize_rows makes them (scale must be NULL);
- *   row_scales NULL:  e4m3 codes e4m3_sat_rne(y * (1 / *scale)), one scale for all (NULL = 1): the operand of the layers above.
+ *   row_scales NULL:  e4m3 codes of y / *scale, one scale for all (NULL = 1): the operand of the layers above.  In fp32 steps
+ *                     e4m3_sat_rne((h * gamma) * (rsqrt(mean(h^2) + eps) / *scale)): the scale is divided into the row's factor.
  * A row whose sum of squares is beyond fp32, or which holds an infinity or a NaN, comes out as NaN: its scale, or its codes. */
 int sl8_rmsnorm_quantize(sl8_handle_t h, const void* x, int dtype, int64_t rows, int cols, int64_t ld,
                          const void* residual, int64_t ld_res, void* sum, int64_t ld_sum,
@@ -344,6 +345,8 @@ int sl8_set_variant(sl8_handle_t h, int variant_id);
 /* Every wait inside the kernels (mbarrier polls) is bounded; a wait that expires records
  * a code in the handle's device status block and the kernel unwinds and exits normally
  * (the reference's mbar_wait spins for ever, kernel_common.cuh:166-178).
+ * What a call whose wait expired was to write is undefined, but for the sum of sl8_rmsnorm_quantize: a row that
+ * did not come keeps what it held, also in place.
  * sl8_device_status synchronises `stream`, reads the block, clears it, and returns SL8_OK
  * or SL8_ERR_DEVICE_TIMEOUT; *detail (optional) receives role, barrier and tile of
  * the first wait that expired. */

@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <map>
 
 #include "sl8_internal.h"
@@ -118,8 +119,8 @@ int cheapest_variant(sl8_handle_t h, CostClass cls, int slot, long long M, int N
 
 int pick_variant(sl8_handle_t h, int op, int out_dtype, long long M, int N, int K, unsigned flags) {
     const int slot = kernel_slot(op, out_dtype);
-    // (1 976 points from 144 to 8 192 wide and 96 to 46 656 rows, int8 and e4m3: these constants pick 0.7 - 1.4 % off the fastest on average,
-    // 17 % at worst from 512 columns on; constants fitted to them would pick 0.8 and 0.7 %)
+    // (siglip_b200/sweeps/b200_scaled.csv, 1 900 points from 144 to 8 192 wide and 96 to 46 656 rows, int8 and e4m3: these constants pick 0.9 - 1.1 % off the
+    // fastest on average, 17 % at worst from 512 columns on; constants fitted to them would pick 0.8 % off)
     if (sl8::op_scaled(op)) return cheapest_variant(h, (flags & SL8_FLAG_NO_ACTIVATION) ? COST_NONE : COST_GELU, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_NO_ACTIVATION)) return cheapest_variant(h, COST_NONE, slot, M, N, K);
     if (op == SL8_OP_FC1_GELU && (flags & SL8_FLAG_GELU_HW_TANH)) return cheapest_variant(h, COST_TANH, slot, M, N, K);
@@ -508,11 +509,15 @@ SL8_API int sl8_destroy(sl8_handle_t h) {
 SL8_API const char* sl8_last_error_string(sl8_handle_t h) {
     if (!h) return g_create_error.c_str();
     // the calling thread's copy: another one may fail, and write the handle's text, while this one reads
-    thread_local std::map<sl8_handle_t, std::string> copies;
-    std::string& copy = copies[h];
-    std::lock_guard<std::mutex> lock(h->err_mu);
-    copy = h->err;
-    return copy.c_str();
+    try {
+        thread_local std::map<sl8_handle_t, std::string> copies;
+        std::string& copy = copies[h];
+        std::lock_guard<std::mutex> lock(h->err_mu);
+        copy = h->err;
+        return copy.c_str();
+    } catch (const std::exception&) {
+        return "out of host memory";
+    }
 }
 
 // =========================================================================== layers

@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(WARP ? kWarpRowThreads : CH == 1 ? 1024 : 512)
 
 // Rows of up to 256 elements (heads, groups), many: LANES lanes to a row, eight elements a lane; its gamma stays in registers.  Bound by the
 // bytes, and by what a row costs besides them (its reductions and divisions): bf16 -> int8 500 000 x 64 23 us (a warp to a row, ring 81), x 128
-// 44 (81); norm with a residual 47 (167) and 89 (167), two rows of a lane at a time (one 53 and 104, four 50 and 94; without the
-// norm one 23, two 25, four 27).  200 000 x 100 bf16, element by element, 29 (53).
+// 44 (81); norm with a residual 47 (167) and 91 (167), two rows of a lane at a time (one 53 and 104, four 50 and 94; without the
+// norm one 23, two 25, four 27).  200 000 x 100 bf16, element by element, 30 (53).
 constexpr int kNarrowThreads = 256;
 __host__ __device__ constexpr int narrow_rows(bool norm, bool vec) { return norm && vec ? 2 : 1; }      // of a lane at a time
 template <typename T, bool NORM, bool VEC, int LANES>
@@ -494,11 +494,11 @@ __device__ __forceinline__ void shared_values(float (&v)[8], const T* p, int lef
 
 // The same for many rows: each block (or, WARP, warp) has a ring of two slots in shared memory and asks for a row, one bulk copy for x and
 // one for the residual, as soon as the one two before it has been read, so that there is always a row on its way and the registers
-// hold one only.  Bound by the bytes: 46 656 x 4 304 bf16 -> int8 92 us, the copy rate of this memory (rows in registers 115);
-// RMS norm of 16 384 x 4 096 with a residual 77 us, 6.1 TB/s (84); 46 656 x 1 152 fp32 -> e4m3 49 us, 5.5 TB/s (65).  Three slots
+// hold one only.  Bound by the bytes: 46 656 x 4 304 bf16 -> int8 93 us, the copy rate of this memory (rows in registers 115);
+// RMS norm of 16 384 x 4 096 with a residual 78 us, 6.0 TB/s (84); 46 656 x 1 152 fp32 -> e4m3 49 us, 5.5 TB/s (65).  Three slots
 // were slower nearly everywhere (16 384 x 4 096 81 us: fewer blocks fit).
 // Rows on any address: the copy takes the 16-byte granules that the row touches, and lanes read consecutive elements from there.  5 003 x 4 305
-// bf16 17.8 us, 3.6 TB/s (from memory, lane by lane, 52: a warp's loads of 64 bytes do not keep enough in flight); the codes go out byte by byte.
+// bf16 18.0 us, 3.6 TB/s (from memory, lane by lane, 52: a warp's loads of 64 bytes do not keep enough in flight); the codes go out byte by byte.
 constexpr int kSlots = 2;
 __host__ __device__ constexpr int gamma_bytes(bool given, int cols) { return given ? (cols + 255) / 256 * 1024 : 0; }
 template <typename T, bool NORM, bool VEC, int CH, bool WARP>
@@ -763,13 +763,14 @@ cudaError_t narrow(int sm_count, cudaStream_t s, const RowArgs& a) {
     return sl8_launch_chained(narrow_row_kernel<T, NORM, VEC, LANES>, static_cast<unsigned>(want < cap ? want : cap), kNarrowThreads, 0, s, a);
 }
 
-// Up to ten rows per SM: a block each, one trip to memory (1 500 x 4 304 bf16 -> int8 5.9 us, ring 6.5); with all eight elements of a
+bool few_rows(int sm_count, const RowArgs& a) { return a.rows <= 10ll * sm_count; }
+
+// Up to ten rows per SM: a block each, one trip to memory (1 500 x 4 304 bf16 -> int8 5.9 us, ring 6.7); with all eight elements of a
 // thread's at once while 256 threads do (norm of one row of 1 152 1.74 us, 1.95 with three times eight), with three from there on (729 x 4 304
 // 3.6 us, 5.4 with one).  Of up to 256 elements: several to a warp.  Up to forty rows per SM, where they are short: a warp each (norm of 5 003 x 1 152 10.3 us, ring 10.9).  Then the ring, by
 // warps while rows are short, by blocks of three times eight elements a thread (100 000 x 512 57 us by warps, 64 by blocks; 20 000 x
-// 2 048 50 either way; 46 656 x 4 304 92, 94 with four, 96 with two), and rows on odd addresses from the tenth row per SM (norm of
+// 2 048 50 either way; 46 656 x 4 304 two us less than with four, four less than with two), and rows on odd addresses from the tenth row per SM (norm of
 // 5 003 x 1 155 15.5 us, in registers 30).
-bool few_rows(int sm_count, const RowArgs& a) { return a.rows <= 10ll * sm_count; }
 template <typename T, bool NORM, bool VEC>
 cudaError_t launch_rows(int sm_count, cudaStream_t s, const RowArgs& a) {
     const bool few = few_rows(sm_count, a);
